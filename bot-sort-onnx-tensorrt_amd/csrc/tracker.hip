@@ -3447,22 +3447,14 @@ int bts_tracker_create(bts_context *ctx, const bts_tracker_config *cfg, bts_trac
     for (int k = 0; ok && k < bts_tracker::RING; ++k) ok = hipEventCreateWithFlags(&t->in_ev[k], hipEventDisableTiming) == hipSuccess;
     ok = ok && hipStreamCreateWithFlags(&t->cs[0], hipStreamNonBlocking) == hipSuccess;
     if (t->cvt_overlap) {
-        if (t->dv.fahead) {
-            // the side passes of BTS_FILTER_AHEAD are background work with a whole step of slack: lowest priority, so that when both
-            // streams have workgroups to place the step's go first
-            int least = 0, greatest = 0;
-            ok = ok && hipDeviceGetStreamPriorityRange(&least, &greatest) == hipSuccess &&
-                 hipStreamCreateWithPriority(&t->side, hipStreamNonBlocking, least) == hipSuccess;
-        } else
+        // (every stream keeps the default priority: work on streams of different priorities can hang on this part)
         ok = ok && hipStreamCreateWithFlags(&t->side, hipStreamNonBlocking) == hipSuccess;
         for (int k = 0; ok && k < 2; ++k)
             ok = hipEventCreateWithFlags(&t->ev_cvt[k], hipEventDisableTiming) == hipSuccess &&
                  hipEventCreateWithFlags(&t->ev_done[k], hipEventDisableTiming) == hipSuccess;
         ok = ok && hipEventCreateWithFlags(&t->ev_in, hipEventDisableTiming) == hipSuccess;
         if (t->dv.smooth_def) {
-            int least = 0, greatest = 0;
-            ok = ok && hipDeviceGetStreamPriorityRange(&least, &greatest) == hipSuccess &&
-                 hipStreamCreateWithPriority(&t->side2, hipStreamNonBlocking, least) == hipSuccess;
+            ok = ok && hipStreamCreateWithFlags(&t->side2, hipStreamNonBlocking) == hipSuccess;
             for (int k = 0; ok && k < 2; ++k) ok = hipEventCreateWithFlags(&t->ev_smooth[k], hipEventDisableTiming) == hipSuccess;
         }
     }
