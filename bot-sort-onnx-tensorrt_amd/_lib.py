@@ -56,6 +56,11 @@ SIGNATURES = {
     "bts_lapjv_exact": (c_int, [_P, _P, c_int, c_int, c_int, c_double, _P, _P, c_int, _P, _P]),
     "bts_feature_ema": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, c_double, _P]),
     "bts_feature_renorm": (c_int, [_P, _P, _P, c_int, c_int, _P]),
+    "bts_mx_row_bytes": (c_int, [c_int, c_int, _P, _P]),
+    "bts_mx_quantize": (c_int, [_P, _P, c_int, c_int, c_int, c_int, c_int, _P, _P, _P]),
+    "bts_mx_dequantize": (c_int, [_P, _P, _P, c_int, c_int, c_int, _P, c_int, c_int, _P]),
+    "bts_rms_norm": (c_int, [_P, c_int, _P, c_int, _P, c_int, _P, c_int, c_int, c_double, _P, c_int, _P, c_int, c_int, _P, _P, _P]),
+    "bts_mx_product": (c_int, [_P, _P, _P, c_int, c_int, _P, _P, c_int, c_int, c_int, c_double, c_int, _P, c_int, c_int, _P]),
     "bts_debug_i8_rows": (c_int, [_P, _P, c_int, c_int, c_double, _P, _P, _P]),
     "bts_debug_i8_pairs": (c_int, [_P, _P, _P, _P, _P, _P, _P, c_int, c_int, _P, _P, _P]),
     "bts_debug_i8_layout": (c_int, [c_int, _P]),

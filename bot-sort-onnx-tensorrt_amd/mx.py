@@ -1,0 +1,181 @@
+"""Microscaled feature rows (csrc/mx.hip): rows in 4 or 8 bits with a scale per 32 elements, the root-mean-square norm that writes
+them, and their product -- `cosine_similarity` for galleries that are kept quantised.
+
+Unlike the NumPy-in / NumPy-out functions of `matching`, everything here takes and returns DEVICE tensors and only enqueues work on
+torch's current stream of their device (like `DeviceTracker.step`): no copies, no synchronisation, safe to capture in a graph.
+"""
+from __future__ import annotations
+
+import ctypes
+
+from . import _lib
+
+_FORMATS = {"e2m1": 0, "e4m3": 1}       # enum bts_mx_format
+_ROW, _BLOCK = 128, 32                  # elements a row is padded to; elements per scale
+
+
+def _dtype_code(dtype):
+    import torch
+    code = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}.get(dtype)      # enum bts_dtype
+    if code is None:
+        raise _lib.BtsError("mx rows: float32, float16 or bfloat16 expected, got %s" % (dtype,))
+    return code
+
+
+def _format_code(fmt):
+    code = _FORMATS.get(fmt)
+    if code is None:
+        raise _lib.BtsError("mx rows: unknown format %r (e2m1, e4m3)" % (fmt,))
+    return code
+
+
+def _rows2d(t, name, like=None):
+    """A device matrix with unit column stride -> (pointer, row stride in elements)."""
+    if not t.is_cuda:
+        raise _lib.BtsError("%s: a device tensor is expected" % name)
+    if t.dim() != 2:
+        raise _lib.BtsError("%s: [rows, d] expected, got %d dimensions" % (name, t.dim()))
+    n, d = t.shape
+    ld = t.stride(0) if n > 1 else max(d, 1)
+    if (t.stride(1) != 1 and d > 1) or ld < d:
+        raise _lib.BtsError("%s: the elements of a row must be adjacent and rows may not overlap (strides %s): call .contiguous()" % (name, tuple(t.stride())))
+    if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
+        raise _lib.BtsError("%s: shape, type and device of x expected (%s %s %s)" % (name, tuple(like.shape), like.dtype, like.device))
+    return t.data_ptr(), ld
+
+
+def _call(device):
+    """(library, context handle, stream) of a device's current stream."""
+    import torch
+    lib = _lib.load()
+    return lib, _lib.default_context(device.index).handle, torch.cuda.current_stream(device).cuda_stream
+
+
+def mx_row_bytes(fmt: str, d: int) -> "tuple[int, int]":
+    """(code bytes, scale bytes) of one row of d elements."""
+    c, s = ctypes.c_int64(), ctypes.c_int64()
+    _lib.check(_lib.load().bts_mx_row_bytes(_format_code(fmt), int(d), ctypes.byref(c), ctypes.byref(s)))
+    return c.value, s.value
+
+
+class MxRows:
+    """n rows of d values in microscaled form: `codes` uint8 [n, code bytes], `scales` uint8 [n, d rounded up to 128, / 32], `fmt`
+    "e2m1" (two elements a byte, the even one in the low nibble) or "e4m3".  Element = code value * 2^(scale - 127); scale 255 = NaN.
+    The layout is include/botsort_hip.h's: a consumer may fill the tensors itself."""
+    __slots__ = ("codes", "scales", "d", "fmt", "_code")
+
+    def __init__(self, codes, scales, d: int, fmt: str):
+        import torch
+        self._code = _format_code(fmt)
+        d = int(d)
+        if d <= 0:
+            raise _lib.BtsError("MxRows: d must be positive")
+        wide = (d + _ROW - 1) // _ROW * _ROW
+        n = codes.shape[0] if codes.dim() == 2 else -1
+        if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.shape != (n, wide // 2 if fmt == "e2m1" else wide)
+                or scales.shape != (n, wide // _BLOCK)):
+            raise _lib.BtsError("MxRows: uint8 codes [n, %d] and scales [n, %d] expected for d = %d in %s, got %s %s" % (
+                wide // 2 if fmt == "e2m1" else wide, wide // _BLOCK, d, fmt, tuple(codes.shape), tuple(scales.shape)))
+        if not codes.is_cuda or codes.device != scales.device:
+            raise _lib.BtsError("MxRows: codes and scales on one GPU expected")
+        if not (codes.is_contiguous() and scales.is_contiguous()):
+            raise _lib.BtsError("MxRows: contiguous codes and scales expected")
+        self.codes, self.scales, self.d, self.fmt = codes, scales, d, fmt
+
+    def __len__(self):
+        return self.codes.shape[0]
+
+    def __repr__(self):
+        return "MxRows(%d x %d, %s, %s)" % (len(self), self.d, self.fmt, self.codes.device)
+
+    @classmethod
+    def empty(cls, n: int, d: int, fmt: str, device="cuda") -> "MxRows":
+        """Room for n rows."""
+        import torch
+        c, s = mx_row_bytes(fmt, d)
+        device = torch.device(device)
+        return cls(torch.empty((int(n), c), dtype=torch.uint8, device=device), torch.empty((int(n), s), dtype=torch.uint8, device=device), d, fmt)
+
+    def dequantize(self, dtype=None):
+        """[n, d] of the values held (float32 unless `dtype` says otherwise)."""
+        import torch
+        dtype = torch.float32 if dtype is None else dtype
+        code = _dtype_code(dtype)
+        n, d = self.codes.shape[0], self.d
+        out = torch.empty((n, d), dtype=dtype, device=self.codes.device)
+        lib, ctx, stream = _call(self.codes.device)
+        _lib.check(lib.bts_mx_dequantize(ctx, self.codes.data_ptr(), self.scales.data_ptr(), self._code, n, d, out.data_ptr(), code, d, stream))
+        return out
+
+
+def _room(out, n, d, fmt, device):
+    if out is None:
+        return MxRows.empty(n, d, fmt, device)
+    if len(out) != n or out.d != d or out.fmt != fmt or out.codes.device != device:
+        raise _lib.BtsError("out: %d x %d rows in %s on %s expected, got %r" % (n, d, fmt, device, out))
+    return out
+
+
+def mx_quantize(x, fmt: str = "e2m1", out: MxRows = None) -> MxRows:
+    """x [n, d] (float32, float16 or bfloat16; rows may be strided) -> its rows in 4 (e2m1) or 8 (e4m3) bits; `out`: rows to fill."""
+    p, ld = _rows2d(x, "x")
+    dt, f = _dtype_code(x.dtype), _format_code(fmt)
+    n, d = x.shape
+    out = _room(out, n, d, fmt, x.device)
+    lib, ctx, stream = _call(x.device)
+    _lib.check(lib.bts_mx_quantize(ctx, p, dt, ld, n, d, f, out.codes.data_ptr(), out.scales.data_ptr(), stream))
+    return out
+
+
+def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4m3", sum_out=None, y_out=None, out: MxRows = None):
+    """Root-mean-square norm of the rows of h = x + residual (rounded to x's type; h = x without a residual), times `weight` [d]
+    -> (rows in `fmt`, h).  fmt=None: no quantised rows, only `y_out`.
+
+    `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` the normalised rows in x's type."""
+    import torch
+    px, ldx = _rows2d(x, "x")
+    dt = _dtype_code(x.dtype)
+    n, d = x.shape
+    pr, ldr = _rows2d(residual, "residual", x) if residual is not None else (None, 0)
+    if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous()):
+        raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
+    if sum_out is None and residual is not None:
+        sum_out = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    ps, lds = _rows2d(sum_out, "sum_out", x) if sum_out is not None else (None, 0)
+    py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
+    if fmt is None and out is not None:
+        raise _lib.BtsError("out: rows to fill need their fmt")
+    f = 0 if fmt is None else _format_code(fmt)
+    rows = None if fmt is None else _room(out, n, d, fmt, x.device)
+    lib, ctx, stream = _call(x.device)
+    _lib.check(lib.bts_rms_norm(ctx, dt, px, ldx, pr, ldr, None if weight is None else weight.data_ptr(), n, d, float(eps), ps, lds, py, ldy, f,
+                                None if rows is None else rows.codes.data_ptr(), None if rows is None else rows.scales.data_ptr(), stream))
+    return rows, x if sum_out is None else sum_out
+
+
+def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = False, dtype=None, out=None):
+    """[len(a), len(b)] of alpha * <a_i, b_j>; floor_zero: max(0, .), the similarity of `cosine_similarity` for unit rows.
+
+    `dtype`: float32 (the default) where both are e2m1; float16 / bfloat16 for any (the default with an e4m3 operand is bfloat16).
+    `out`: a matrix to fill (its type counts; rows may be strided)."""
+    import torch
+    if not isinstance(a, MxRows) or not isinstance(b, MxRows):
+        raise _lib.BtsError("mx_product: MxRows expected")
+    device = a.codes.device
+    if a.d != b.d or b.codes.device != device:
+        raise _lib.BtsError("mx_product: rows of one width on one device expected, got %r and %r" % (a, b))
+    n, m = a.codes.shape[0], b.codes.shape[0]
+    if out is None:
+        if dtype is None:
+            dtype = torch.float32 if a.fmt == b.fmt == "e2m1" else torch.bfloat16
+        code = _dtype_code(dtype)
+        out = torch.empty((n, m), dtype=dtype, device=device)
+    else:
+        code = _dtype_code(out.dtype)
+        if tuple(out.shape) != (n, m) or out.device != device or dtype not in (None, out.dtype):
+            raise _lib.BtsError("out: [%d, %d] on %s%s expected" % (n, m, device, "" if dtype is None else " of %s" % dtype))
+    po, ld = _rows2d(out, "out")
+    lib, ctx, stream = _call(device)
+    _lib.check(lib.bts_mx_product(ctx, a.codes.data_ptr(), a.scales.data_ptr(), a._code, n, b.codes.data_ptr(), b.scales.data_ptr(), b._code,
+                                  m, a.d, float(alpha), 1 if floor_zero else 0, po, code, ld, stream))
+    return out

@@ -159,6 +159,47 @@ int bts_feature_ema(bts_context *ctx, float *curr, float *smooth, uint8_t *has_s
  * feats[idx[q], :] /= ||.||_2 for q in [0,k) (idx nullable = identity). */
 int bts_feature_renorm(bts_context *ctx, float *feats, const int32_t *idx, int k, int d, bts_stream stream);
 
+/* ------------------------------------------------------------------------------ microscaled feature rows
+ *
+ * Rows in 4 or 8 bits with a scale per 32 elements: a gallery of feature rows in an eighth of its float32 size, and their
+ * products straight on the matrix cores.  A row of d values is held as
+ *   codes[code_bytes]    BTS_MX_E2M1: two elements a byte, the even one in the low nibble (values 0 .5 1 1.5 2 3 4 6 and a sign);
+ *                        BTS_MX_E4M3: one a byte (up to 448, smallest step 2^-9)
+ *   scales[scale_bytes]  one byte s per 32 elements, worth 2^(s - 127); 255 = the whole block is NaN
+ * zero-padded to a multiple of 128 elements; rows follow each other without gaps.  codes: 16-byte, scales: 4-byte aligned.
+ * Quantisation (OCP microscaling formats): s = 127 + clamp(floor(log2(max |v|)) - emax, -127, 127), emax = 2 (E2M1) / 8 (E4M3),
+ * elements v / 2^(s - 127) rounded to nearest even, saturating.  A block with an infinity or a NaN in it becomes NaN.
+ * Types of x / out / y: BTS_F32, BTS_F16 or BTS_BF16 (enum bts_dtype); row strides (ld*) are in elements, >= d. */
+enum bts_mx_format { BTS_MX_E2M1 = 0, BTS_MX_E4M3 = 1 };
+
+/* Bytes of one row's codes and scales (host-only). */
+int bts_mx_row_bytes(int format, int d, int64_t *code_bytes, int64_t *scale_bytes);
+
+/* x[n,d] -> codes, scales (the padding included). */
+int bts_mx_quantize(bts_context *ctx, const void *x, int x_dtype, int ldx, int n, int d, int format,
+                    uint8_t *codes, uint8_t *scales, bts_stream stream);
+
+/* codes, scales -> out[n,d], the values they stand for, rounded once to out's type. */
+int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *scales, int format, int n, int d,
+                      void *out, int out_dtype, int ldo, bts_stream stream);
+
+/* Root-mean-square norm of rows, with the residual's addition and a quantised output:
+ *   h = x + residual, rounded to `dtype` (h = x without a residual);   v = h / sqrt(mean(h^2) + eps) * weight
+ * sum (nullable) = h; y (nullable) = v in `dtype`; codes / scales (both nullable) = v in `format`, quantised from float32.
+ * residual[n,d] and weight[d] are nullable, all of x's type.  sum and y may be x or residual themselves (same row stride), not
+ * each other.  The mean is taken in float32: rows whose sum of squares passes its range are outside.  eps > 0. */
+int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void *residual, int ldr,
+                 const void *weight, int n, int d, double eps, void *sum, int lds, void *y, int ldy,
+                 int format, uint8_t *codes, uint8_t *scales, bts_stream stream);
+
+/* out[i*ld+j] = alpha * <a_i, b_j>, optionally max(0, .) (floor_zero != 0; a NaN stays one): bts_cos_similarity on microscaled
+ * rows.  a: n rows, b: m rows, of the same d; formats may differ.  Products are formed exactly and added in float32 where both are
+ * E2M1; the matrix instruction aligns the products of an E4M3 operand to the largest of them with about 13 bits behind it, so
+ * out_dtype BTS_F32 needs two E2M1 operands and the 16-bit types take any. */
+int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_scales, int a_format, int n,
+                   const uint8_t *b_codes, const uint8_t *b_scales, int b_format, int m, int d, double alpha,
+                   int floor_zero, void *out, int out_dtype, int ld, bts_stream stream);
+
 /* remove_duplicate_stracks, D:1665-1680: drop_a[n] / drop_b[m] flags (uint8, overwritten) for
  * pairs with 1-IoU < thresh; age_* = frame_id - start_frame. */
 int bts_dedupe_pairs(bts_context *ctx, const double *a_tlbr, const uint8_t *a_f32, const int32_t *age_a,
@@ -262,7 +303,7 @@ typedef struct bts_tracker_config {
                                    handed to the solver -- config 5's "fp16 cost matrix" (this design has no matrix to store:
                                    the rounding is what the mode means for the results).  Needs tie_mode 0 */
 } bts_tracker_config;
-enum bts_dtype { BTS_F64 = 0, BTS_F32 = 1, BTS_F16 = 2 };
+enum bts_dtype { BTS_F64 = 0, BTS_F32 = 1, BTS_F16 = 2, BTS_BF16 = 3 /* mx rows only */ };
 
 /* sizeof(bts_tracker_config) in THIS library.  A binding in another language checks its mirror of the struct against it
    BEFORE it hands a buffer to bts_tracker_default_config (which writes that many bytes). */

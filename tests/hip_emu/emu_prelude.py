@@ -49,6 +49,7 @@ torch.cuda.set_stream = lambda s: None
 torch.cuda.stream = lambda s: _Stream()
 torch.cuda.Event = _Event
 torch.Tensor.cuda = lambda self, *a, **k: self.clone()       # (a host -> device copy is a COPY: kernels must not write into the caller's array)
+torch.Tensor.is_cuda = property(lambda self: True)           # (entry points that take device tensors check it)
 _to = torch.Tensor.to
 
 

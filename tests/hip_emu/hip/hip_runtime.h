@@ -72,7 +72,7 @@ enum Op { OP_SHFL, OP_SHFL_XOR, OP_SHFL_UP, OP_BALLOT, OP_READLANE, OP_READFIRST
 uint64_t collective(Op op, int site, uint64_t value, int arg, int arg2, uint64_t old_value);
 // operand exchange of a matrix instruction: every participating lane deposits `n` <= GATHER_MAX bytes; returns the wavefront's
 // staging area [64][GATHER_MAX] (lanes that do not take part read as zero), valid until the wavefront's next gather
-constexpr int GATHER_MAX = 64;
+constexpr int GATHER_MAX = 80;
 const char *gather(int site, const void *mine, int n);
 }  // namespace emu
 
@@ -193,6 +193,63 @@ static inline emu_f32x16 emu_mfma_f32_32x32x2f32(int site, float a, float b, emu
     return c;
 }
 #define __builtin_amdgcn_mfma_f32_32x32x2f32(a, b, c, x, y, z) emu_mfma_f32_32x32x2f32(__COUNTER__, (a), (b), (c))
+// v_mfma_scale_f32_16x16x128_f8f6f4, formats 0 (e4m3) and 4 (e2m1): lane l supplies row l & 15 of either operand.  With g = l >> 4 an
+// e2m1 operand's 16 bytes are elements 32 g .. 32 g + 31 (even one in the low nibble), an e4m3 operand's 32 bytes are elements
+// 16 g .. + 15 and 64 + 16 g .. + 15; scale byte `op_sel` of lane group g belongs to elements 32 g .. 32 g + 31 (255: NaN).  Lane l receives
+// D[4 (l >> 4) + r][l & 15] in c[r].  (Maps and NaN checked on hardware.)  The sum is taken in double and rounded once: the hardware's own
+// alignment of e4m3 products is not modelled.
+typedef int emu_v8i __attribute__((ext_vector_type(8)));
+typedef float emu_f32x4 __attribute__((ext_vector_type(4)));
+static inline double emu_f8f6f4(int fmt, int code) {
+    if (fmt == 4) { static const double t[8] = {0, 0.5, 1, 1.5, 2, 3, 4, 6}; return code & 8 ? -t[code & 7] : t[code & 7]; }
+    const int e = (code >> 3) & 15, f = code & 7;
+    if ((code & 127) == 127) return NAN;
+    const double v = e ? ldexp(8.0 + f, e - 10) : ldexp((double)f, -9);
+    return code & 128 ? -v : v;
+}
+static inline emu_f32x4 emu_mfma_scale_16x16x128(int site, emu_v8i a, emu_v8i b, emu_f32x4 c, int fa, int fb, int oa, int sa, int ob, int sb) {
+    struct { emu_v8i a, b; int sa, sb; } mine = {a, b, (sa >> (8 * oa)) & 255, (sb >> (8 * ob)) & 255};
+    const char *all = emu::gather(site, &mine, 72);
+    const int lane = (int)(emu::tid_x() & 63), j = lane & 15, q = lane >> 4;
+    auto element = [&](int fmt, int operand, int row, int k) {
+        const int g = fmt == 4 ? k / 32 : (k % 64) / 16, at = fmt == 4 ? (k % 32) / 2 : (k / 64) * 16 + k % 16;
+        const unsigned char *p = (const unsigned char *)(all + (row + 16 * g) * emu::GATHER_MAX + 32 * operand);
+        const int code = fmt == 4 ? (p[at] >> (4 * (k & 1))) & 15 : p[at];
+        int s;
+        memcpy(&s, all + (row + 16 * (k / 32)) * emu::GATHER_MAX + 64 + 4 * operand, 4);
+        return emu_f8f6f4(fmt, code) * (s == 255 ? (double)NAN : ldexp(1.0, s - 127));
+    };
+    for (int r = 0; r < 4; ++r) {
+        double sum = c[r];
+        for (int k = 0; k < 128; ++k) sum += element(fa, 0, 4 * q + r, k) * element(fb, 1, j, k);
+        c[r] = (float)sum;
+    }
+    return c;
+}
+#define __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(a, b, c, fa, fb, oa, sa, ob, sb) emu_mfma_scale_16x16x128(__COUNTER__, (a), (b), (c), (fa), (fb), (oa), (sa), (ob), (sb))
+// conversions to e2m1 / e4m3: nearest, ties to the even code; e2m1 saturates, e4m3 above 464 is NaN (the kernels clamp first)
+static inline int emu_to_f8f6f4(int fmt, float v) {
+    const int n = fmt == 4 ? 8 : 127;
+    const double a = fabs((double)v);
+    int best = 0;
+    double gap = INFINITY;
+    for (int code = 0; code < n; ++code) {
+        const double g = fabs(emu_f8f6f4(fmt, code) - a);
+        if (g < gap || (g == gap && !(code & 1))) { gap = g; best = code; }
+    }
+    if (v != v || (fmt == 0 && a > 464)) best = fmt == 0 ? 127 : 7;
+    return best | (signbit(v) ? (fmt == 4 ? 8 : 128) : 0);
+}
+static inline unsigned emu_cvt_pk_fp4(unsigned old, float a, float b, float scale, int sel) {
+    const unsigned byte = (unsigned)(emu_to_f8f6f4(4, a / scale) | emu_to_f8f6f4(4, b / scale) << 4);
+    return (old & ~(0xffu << (8 * sel))) | byte << (8 * sel);
+}
+static inline int emu_cvt_pk_fp8(float a, float b, int old, bool high) {
+    const unsigned half = (unsigned)(emu_to_f8f6f4(0, a) | emu_to_f8f6f4(0, b) << 8);
+    return (int)(high ? ((unsigned)old & 0xffffu) | half << 16 : ((unsigned)old & 0xffff0000u) | half);
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, scale, sel) emu_cvt_pk_fp4((old), (a), (b), (scale), (sel))
+#define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, high) emu_cvt_pk_fp8((a), (b), (old), (high))
 // (only named inside a discarded `if constexpr` branch of a timing experiment)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, ...) (c)
 // global_load_lds (16 B per lane): the LDS image is lane-linear from the wave-uniform base -- lane l's bytes land at base + 16 l.

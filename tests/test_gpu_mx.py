@@ -1,0 +1,529 @@
+"""Microscaled feature rows (csrc/mx.hip) against their definition in float64: quantisation and decoding bit for bit, the
+root-mean-square norm and the product within bounds that are derived where they stand."""
+import itertools
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+EMAX = {"e2m1": 2, "e4m3": 8}
+DTYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+HALF = {"f32": 2.0 ** -24, "f16": 2.0 ** -11, "bf16": 2.0 ** -8}       # half a step, relative to the value
+
+
+@pytest.fixture(scope="module")
+def bts():
+    import importlib
+    return importlib.import_module("bot-sort-onnx-tensorrt_amd")
+
+
+# ------------------------------------------------------------------------------------------------------- definition, float64
+
+def grid(fmt):
+    """non-negative values in the order of their codes"""
+    if fmt == "e2m1":
+        return np.array([0, 0.5, 1, 1.5, 2, 3, 4, 6])
+    return np.array([(m / 8) * 2.0 ** -6 if e == 0 else (1 + m / 8) * 2.0 ** (e - 7) for e in range(16) for m in range(8)][:127])
+
+
+def wide(d):
+    return (d + 127) // 128 * 128
+
+
+def blocks(v, d):
+    out = np.zeros((v.shape[0], wide(d)))
+    out[:, :d] = v
+    return out.reshape(v.shape[0], -1, 32)
+
+
+def quantize_ref(v, fmt):
+    """float64 [n, d] -> (codes [n, wide] one per element, scales [n, wide / 32])"""
+    b = blocks(v, v.shape[1])
+    bad = ~np.isfinite(b).all(-1)
+    top = np.where(bad, 0, np.abs(b).max(-1))
+    e = np.where(top > 0, np.frexp(top)[1] - 1, -1000) - EMAX[fmt]
+    s = np.where(bad, 255, np.clip(e, -127, 127) + 127)
+    x = np.where(bad[..., None], 0, b) / np.exp2(np.where(bad, 0, s - 127.0))[..., None]
+    g, a = grid(fmt), np.abs(x)
+    hi = np.minimum(np.searchsorted(g, a), len(g) - 1)
+    lo = np.maximum(hi - 1, 0)
+    code = np.where(a - g[lo] < g[hi] - a, lo, np.where(a - g[lo] > g[hi] - a, hi, np.where(lo % 2 == 0, lo, hi)))
+    code = code + np.where(np.signbit(x), 8 if fmt == "e2m1" else 128, 0)
+    return code.reshape(v.shape[0], -1), s
+
+
+def pack(code, fmt):
+    return (code[:, 0::2] + 16 * code[:, 1::2] if fmt == "e2m1" else code).astype(np.uint8)
+
+
+def unpack(codes, fmt):
+    return np.stack((codes & 15, codes >> 4), -1).reshape(codes.shape[0], -1) if fmt == "e2m1" else codes
+
+
+def decode_ref(codes, scales, fmt):
+    """packed codes, scales -> float64 [n, wide]"""
+    g = grid(fmt)
+    t = np.concatenate((g, -g)) if fmt == "e2m1" else np.concatenate((g, [np.nan], -g, [np.nan]))
+    s = scales.astype(np.float64)
+    return t[unpack(codes, fmt)] * np.repeat(np.where(s == 255, np.nan, np.exp2(s - 127)), 32, axis=1)
+
+
+def host(rows):
+    return rows.codes.cpu().numpy(), rows.scales.cpu().numpy()
+
+
+def rows_of(bts, v, fmt):
+    """float64 values -> MxRows filled from the definition, and the values they stand for"""
+    code, s = quantize_ref(v, fmt)
+    c = pack(code, fmt)
+    r = bts.MxRows(torch.from_numpy(c).cuda(), torch.from_numpy(s.astype(np.uint8)).cuda(), v.shape[1], fmt)
+    return r, decode_ref(c, s, fmt)
+
+
+# ------------------------------------------------------------------------------------------------------------- quantisation
+
+def awkward(n, d, dtype, seed):
+    """values with ties, powers of two, subnormals, zeros, huge and tiny rows, exactly representable in dtype"""
+    r = np.random.default_rng(seed)
+    x = r.standard_normal((n, d)) * np.exp2(r.integers(-12, 12, (n, 1)))
+    kind = r.integers(0, 6, (n, d))
+    x = np.where(kind == 0, r.integers(-64, 65, (n, d)) / 8.0, x)                # ties and exact values
+    x = np.where(kind == 1, np.sign(x) * np.exp2(r.integers(-8, 9, (n, d))), x)
+    x = np.where(kind == 2, 0.0, x)
+    t = DTYPES[dtype]
+    if n > 2:
+        x[1] = 0.0
+        x[2] *= float(torch.finfo(t).tiny) * 2.0 ** -3                             # subnormals of the type
+        x[n - 1] = np.sign(x[n - 1]) * float(torch.finfo(t).max)
+    return torch.from_numpy(x).to(t)
+
+
+SHAPES = [(1, 1), (1, 31), (3, 32), (5, 33), (4, 127), (7, 128), (2, 129), (9, 384), (3, 1111), (33, 250), (300, 96)]
+
+
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+@pytest.mark.parametrize("n,d", SHAPES)
+def test_quantize_and_back(bts, n, d, fmt, dtype):
+    x = awkward(n, d, dtype, 17 * n + d)
+    code, s = quantize_ref(x.double().numpy(), fmt)
+    q = bts.mx_quantize(x.cuda(), fmt)
+    c, sc = host(q)
+    assert np.array_equal(sc, s)
+    assert np.array_equal(c, pack(code, fmt))
+    want = decode_ref(c, sc, fmt)[:, :d]
+    for out in DTYPES:
+        got = q.dequantize(DTYPES[out]).cpu()
+        # the values have at most 4 significant bits: one rounding, from float32 on (products below its range round there first)
+        assert torch.equal(got, torch.from_numpy(want).float().to(DTYPES[out])), out
+    assert len(q) == n and q.d == d
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+def test_quantize_non_finite_blocks(bts, fmt):
+    x = awkward(6, 200, "f32", 3)
+    x[0, 5] = float("inf"); x[1, 40] = float("-inf"); x[2, 199] = float("nan"); x[3, 0] = float("nan"); x[3, 1] = float("inf"); x[5, 128:160] = float("inf")
+    code, s = quantize_ref(x.double().numpy(), fmt)
+    assert (s == 255).sum() == 5
+    q = bts.mx_quantize(x.cuda(), fmt)
+    c, sc = host(q)
+    assert np.array_equal(sc, s)
+    ok = np.repeat(s != 255, 32, axis=1)
+    assert np.array_equal(unpack(c, fmt)[ok], code[ok]) and (unpack(c, fmt)[~ok] % (8 if fmt == "e2m1" else 128) == 0).all()
+    assert np.array_equal(np.isnan(q.dequantize().cpu().numpy()), ~ok[:, :200])
+
+
+@pytest.mark.parametrize("dtype,off,ld", [("f32", 0, 260), ("f32", 1, 263), ("bf16", 0, 264), ("bf16", 3, 259), ("f16", 8, 264)])
+def test_quantize_strided_rows(bts, dtype, off, ld):
+    """rows inside a wider matrix, aligned for wide loads or not; the matrix is left as it was"""
+    n, d = 13, 250
+    flat = awkward(1, off + n * ld, dtype, off + ld)[0]
+    dev = flat.cuda()
+    x = torch.as_strided(dev, (n, d), (ld, 1), off)
+    ref = torch.as_strided(flat, (n, d), (ld, 1), off)
+    q = bts.mx_quantize(x, "e4m3")
+    code, s = quantize_ref(ref.double().numpy(), "e4m3")
+    assert np.array_equal(host(q)[0], pack(code, "e4m3")) and np.array_equal(host(q)[1], s)
+    assert torch.equal(dev.cpu().view(torch.uint8), flat.view(torch.uint8))
+
+
+@pytest.mark.parametrize("fmt", ["e2m1", "e4m3"])
+def test_dequantize_every_code_and_scale(bts, fmt):
+    per = 16 if fmt == "e2m1" else 256
+    code = np.tile(np.arange(per), (256, 256 // per))
+    s = np.tile(np.arange(256)[:, None], (1, 8))
+    r = bts.MxRows(torch.from_numpy(pack(code, fmt)).cuda(), torch.from_numpy(s.astype(np.uint8)).cuda(), 256, fmt)
+    with np.errstate(over="ignore"):
+        want = decode_ref(pack(code, fmt), s, fmt).astype(np.float32)
+    got = r.dequantize().cpu().numpy()
+    assert np.array_equal(got, want, equal_nan=True)
+    for t in (torch.float16, torch.bfloat16):
+        assert torch.equal(r.dequantize(t).cpu().nan_to_num(nan=12345.0), torch.from_numpy(want).to(t).nan_to_num(nan=12345.0))
+
+
+def test_rows_behind_the_last_stay(bts):
+    """out rows of a larger buffer: only the rows given are written, by every operator"""
+    x = awkward(5, 70, "f32", 9).cuda()
+    room = bts.MxRows.empty(8, 70, "e2m1")
+    room.codes.fill_(0xAB); room.scales.fill_(0xCD)
+    view = bts.MxRows(room.codes[:5], room.scales[:5], 70, "e2m1")
+    bts.mx_quantize(x, "e2m1", out=view)
+    bts.rms_norm_mx(x, fmt="e2m1", out=view)
+    assert (room.codes[5:].cpu() == 0xAB).all() and (room.scales[5:].cpu() == 0xCD).all()
+    out = torch.full((8, 16), 7.0).cuda()
+    bts.mx_product(view, view, out=out[:5, :5])
+    o = out.cpu()
+    assert (o[5:] == 7).all() and (o[:5, 5:] == 7).all() and (o[:5, :5] != 7).any()
+
+
+# ------------------------------------------------------------------------------------------------------------------- norm
+
+def norm_ref(x, residual, weight, eps):
+    """(h as stored, v float64)"""
+    h = x if residual is None else (x.double() + residual.double()).to(x.dtype)
+    f = h.double().numpy()
+    v = f / np.sqrt((f * f).mean(-1, keepdims=True) + eps)
+    return h, v if weight is None else v * weight.double().numpy()
+
+
+def norm_delta(d):
+    """relative error of the float32 computation: the sum of squares is a chain of at most 8 * ceil(d / 512) fused steps per lane and 9
+    more in the reduction (half of it counts, through the root), the mean's division, the root, the reciprocal and two products"""
+    return (0.5 * (8 * math.ceil(d / 512) + 9) + 5) * 2.0 ** -24
+
+
+def check_quantized(v, codes, scales, fmt, d, delta):
+    """codes are a correct quantisation of values within `delta` of v"""
+    b, s = blocks(v, d), scales.astype(np.int64)
+    top = np.abs(b).max(-1)
+
+    def byte(t):
+        return np.clip(np.where(t > 0, np.frexp(t)[1] - 1, -1000) - EMAX[fmt], -127, 127) + 127
+    assert ((s == byte(top * (1 - delta))) | (s == byte(top * (1 + delta)))).all()
+    unit = np.exp2(s - 127.0)[..., None]
+    x = np.abs(b) / unit
+    mant, emin, most = (1, 0, 6.0) if fmt == "e2m1" else (3, -6, 448.0)
+    e = np.maximum(np.where(x > 0, np.frexp(x)[1] - 1, -1000), emin)
+    half = np.exp2(e - mant - 1.0)                                                  # half a step of the element's binade
+    q = decode_ref(codes, scales, fmt).reshape(b.shape) / unit
+    err = np.abs(np.abs(q) - np.minimum(x, most))
+    assert (err <= half + delta * x).all(), float((err - half - delta * x).max())
+    assert ((q == 0) | (np.sign(q) == np.sign(b))).all()
+
+
+NORM_SHAPES = [(1, 1), (1, 2048), (3, 31), (5, 128), (2, 257), (17, 384), (4, 1111), (3, 2056), (2, 4096), (2, 8200)]
+
+
+@pytest.mark.parametrize("residual,weight", [(False, False), (True, True), (True, False), (False, True)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,d", NORM_SHAPES)
+def test_rms_norm(bts, n, d, dtype, residual, weight):
+    t, r = DTYPES[dtype], np.random.default_rng(d)
+    x = torch.from_numpy(r.standard_normal((n, d)) * np.exp2(r.integers(-4, 5, (n, 1)))).to(t)
+    res = torch.from_numpy(r.standard_normal((n, d))).to(t) if residual else None
+    w = torch.from_numpy(1 + 0.2 * r.standard_normal(d)).to(t) if weight else None
+    dev = lambda a: None if a is None else a.cuda()  # noqa: E731
+    for fmt in ("e4m3", "e2m1", None):
+        y = torch.full((n, d), 9.0, dtype=t).cuda()
+        xd, rd = x.cuda(), dev(res)
+        q, h = bts.rms_norm_mx(xd, residual=rd, weight=dev(w), eps=1e-5, fmt=fmt, y_out=y)
+        want_h, v = norm_ref(x, res, w, 1e-5)
+        assert torch.equal(h.cpu(), want_h)
+        assert torch.equal(xd.cpu(), x) and (rd is None or torch.equal(rd.cpu(), res))
+        delta = norm_delta(d)
+        # a value below the type's normal range is off by half of its smallest step
+        tol = (delta + HALF[dtype] * (1 + delta)) * np.abs(v) + float(torch.finfo(t).smallest_normal) * HALF[dtype]
+        assert (np.abs(y.cpu().double().numpy() - v) <= tol).all()
+        if fmt is None:
+            assert q is None
+        else:
+            check_quantized(v, *host(q), fmt, d, delta)
+
+
+@pytest.mark.parametrize("d", [96, 5000, 9000])
+def test_rms_norm_in_place(bts, d):
+    x = awkward(6, d, "bf16", d)
+    res = awkward(6, d, "bf16", d + 1)
+    x[5] = 1.0; res[5] = -1.0                                                       # (the type's largest values would pass float32's range)
+    q0, h0 = bts.rms_norm_mx(x.cuda(), residual=res.cuda(), fmt="e4m3")
+    for into in ("x", "residual"):
+        xd, rd = x.cuda(), res.cuda()
+        q, h = bts.rms_norm_mx(xd, residual=rd, fmt="e4m3", sum_out=xd if into == "x" else rd)
+        assert h is (xd if into == "x" else rd) and torch.equal(h.cpu(), h0.cpu())
+        assert torch.equal(q.codes.cpu(), q0.codes.cpu()) and torch.equal(q.scales.cpu(), q0.scales.cpu())
+        assert torch.equal((rd if into == "x" else xd).cpu(), res if into == "x" else x)
+    y0 = torch.empty_like(x).cuda()
+    bts.rms_norm_mx(x.cuda(), residual=res.cuda(), fmt=None, y_out=y0)
+    xd = x.cuda()
+    bts.rms_norm_mx(xd, residual=res.cuda(), fmt=None, y_out=xd)                     # the normalised rows in the place of x
+    assert torch.equal(xd.cpu(), y0.cpu())
+
+
+def test_rms_norm_zero_and_non_finite_rows(bts):
+    x = torch.ones((5, 300))
+    x[1] = 0; x[2, 7] = float("inf"); x[3, 70] = float("nan")
+    q, _ = bts.rms_norm_mx(x.cuda(), fmt="e4m3")
+    v = q.dequantize().cpu().numpy()
+    # 1 / sqrt(1 + 1e-6) = 0.9999995 is below 1: its block's exponent is -1, its unit 2^(-1 - 8), and 0.9999995 * 512 = 511.9997
+    # saturates at 448: the value held is 448 / 512
+    assert (v[0] == 0.875).all() and (v[4] == 0.875).all() and (v[1] == 0).all()
+    assert np.isnan(v[3]).all()                                                     # a NaN takes the row's norm with it
+    assert np.isnan(v[2, :32]).all() and (v[2, 32:] == 0).all()                     # inf / inf in its block, x / inf elsewhere
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rms_norm_strided(bts, dtype):
+    t = DTYPES[dtype]
+    big = awkward(12, 700, dtype, 5).clamp(-100, 100)
+    x, res = big[:, 3:403], big[:, 290:690]
+    dev = big.cuda()
+    out = torch.zeros((12, 500), dtype=t).cuda()
+    q, h = bts.rms_norm_mx(dev[:, 3:403], residual=dev[:, 290:690], sum_out=out[:, 50:450], fmt="e2m1")
+    want, v = norm_ref(x, res, None, 1e-6)
+    assert torch.equal(out[:, 50:450].cpu(), want) and (out[:, :50].cpu() == 0).all() and (out[:, 450:].cpu() == 0).all()
+    check_quantized(v, *host(q), "e2m1", 400, norm_delta(400))
+
+
+# ----------------------------------------------------------------------------------------------------------------- product
+
+def product_bound(a, b, out, ref, fmts):
+    """half a step of the output's type, and the sum's own error: with two E2M1 operands products are exact and at most one float32
+    rounding falls on each partial sum (instructions, parts of the row and the factor: d / 128 + 20), each at most 2^-24 of the sum
+    of magnitudes; with an E4M3 operand the instruction's alignment leaves 2^-12 of that sum"""
+    mag = np.abs(a) @ np.abs(b).T
+    own = (a.shape[1] / 128 + 20) * 2.0 ** -24 if fmts == ("e2m1", "e2m1") else 2.0 ** -12
+    return HALF[out] * np.abs(ref) + own * mag + float(torch.finfo(DTYPES[out]).smallest_normal) * HALF[out]
+
+
+def feature_rows(n, d, seed):
+    r = np.random.default_rng(seed)
+    v = r.standard_normal((n, d)) * np.exp(0.5 * r.standard_normal(d))
+    return v * np.exp2(r.integers(-3, 4, (n, 1)))
+
+
+FMTS = list(itertools.product(["e2m1", "e4m3"], ["e2m1", "e4m3"]))
+PRODUCTS = [(1, 1, 1), (1, 300, 64), (16, 17, 128), (17, 1, 300), (33, 65, 500), (5, 130, 1111), (64, 64, 256), (100, 37, 129)]
+BIG = [(1, 5000, 2048), (3, 70001, 96), (40, 2000, 1024), (200, 333, 4100), (512, 256, 256), (777, 1300, 640), (1500, 1025, 2048), (2500, 4, 512), (33000, 40, 200)]
+
+
+def run_product(bts, n, m, d, fa, fb, out):
+    va, vb = feature_rows(n, d, 3 * n + d), feature_rows(m, d, 5 * m + d)
+    if n > 3:
+        va[2] = 0.0
+    a, ra = rows_of(bts, va, fa)
+    b, rb = rows_of(bts, vb, fb)
+    ref = ra @ rb.T
+    for alpha, floor in ((1.0, False), (0.125, True)):
+        want = np.maximum(ref * alpha, 0) if floor else ref * alpha
+        got = bts.mx_product(a, b, alpha=alpha, floor_zero=floor, dtype=DTYPES[out]).cpu().double().numpy()
+        assert got.shape == (n, m)
+        tol = product_bound(ra, rb, out, want, (fa, fb)) * (1 if alpha == 1 else alpha if out == "f32" else 1)
+        assert (np.abs(got - want) <= tol).all(), float((np.abs(got - want) / np.maximum(tol, 1e-300)).max())
+        if n > 3:
+            assert (got[2] == 0).all()
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m,d", PRODUCTS)
+def test_product(bts, n, m, d, fa, fb):
+    for out in (["f32", "bf16"] if fa == fb == "e2m1" else ["f16", "bf16"]):
+        run_product(bts, n, m, d, fa, fb, out)
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m,d", BIG)
+def test_product_big(bts, n, m, d, fa, fb):
+    run_product(bts, n, m, d, fa, fb, "f32" if fa == fb == "e2m1" else "bf16")
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m", [(20, 40), (1, 700), (300, 290)])
+def test_product_nan_blocks_and_extreme_scales(bts, n, m, fa, fb):
+    d = 200
+    va, vb = feature_rows(n, d, 1), feature_rows(m, d, 2)
+    a, ra = rows_of(bts, va, fa)
+    b, rb = rows_of(bts, vb, fb)
+    a.scales[n - 1, 2] = 255                       # a NaN block takes its row (and the other operand's column) with it
+    b.scales[3, 0] = 255
+    a.scales[0, 7:] = 254                          # the padding (elements 224 ..): zero whatever its scale says
+    b.scales[m - 1] = 0                            # 2^-127: products around the end of float32's range
+    got = bts.mx_product(a, b, dtype=torch.bfloat16, floor_zero=True).cpu().double().numpy()
+    nan = np.zeros((n, m), bool)
+    nan[n - 1] = True; nan[:, 3] = True
+    assert np.array_equal(np.isnan(got), nan)
+    ra, rb = (np.nan_to_num(decode_ref(*host(r), r.fmt)) for r in (a, b))
+    ref = np.maximum(ra @ rb.T, 0)
+    tol = product_bound(ra, rb, "bf16", ref, (fa, fb)) + 256 * 2.0 ** -126           # (a product below the normal range may count as 0)
+    assert (np.abs(got - ref) <= tol)[~nan].all()
+
+
+@pytest.mark.parametrize("out", list(DTYPES))
+@pytest.mark.parametrize("n,m,ld,off", [(7, 37, 61, 0), (7, 37, 64, 1), (130, 132, 140, 4), (130, 131, 133, 2)])
+def test_product_into_a_wider_matrix(bts, n, m, ld, off, out):
+    """unaligned and aligned rows of the output; what lies between the rows is left alone"""
+    a, ra = rows_of(bts, feature_rows(n, 160, 4), "e2m1")
+    b, rb = rows_of(bts, feature_rows(m, 160, 5), "e2m1")
+    flat = torch.full((off + n * ld + 5,), 3.0, dtype=DTYPES[out]).cuda()
+    view = torch.as_strided(flat, (n, m), (ld, 1), off)
+    assert bts.mx_product(a, b, out=view) is view
+    want = bts.mx_product(a, b, dtype=DTYPES[out]).cpu()
+    got = flat.cpu()
+    assert torch.equal(torch.as_strided(got, (n, m), (ld, 1), off), want)
+    mask = torch.ones_like(got, dtype=torch.bool)
+    torch.as_strided(mask, (n, m), (ld, 1), off)[...] = False
+    assert (got[mask] == 3).all()
+
+
+def test_empty_sides(bts):
+    e, one = bts.MxRows.empty(0, 100, "e2m1"), bts.mx_quantize(torch.ones((1, 100)).cuda(), "e2m1")
+    assert bts.mx_product(e, one).shape == (0, 1) and bts.mx_product(one, e).shape == (1, 0)
+    assert len(bts.mx_quantize(torch.ones((0, 100)).cuda())) == 0 and e.dequantize().shape == (0, 100)
+    q, h = bts.rms_norm_mx(torch.ones((0, 100)).cuda())
+    assert len(q) == 0 and h.shape == (0, 100)
+
+
+# ----------------------------------------------------------------------------------------------------------------- together
+
+@pytest.mark.parametrize("gallery,queries,d,fa,fmt", [(200, 33, 384, "e2m1", "e4m3"), (130, 1, 250, "e2m1", "e2m1"), (64, 70, 512, "e4m3", "e4m3")])
+def test_gallery_search_as_it_is_used(bts, gallery, queries, d, fa, fmt):
+    """enrol a gallery in few bits; normalise a frame's rows (residual, weight) to few bits; their cosine similarities.  Every stage is
+    held to the one before it, and the end to `cosine_similarity` of the unquantised unit rows."""
+    g = feature_rows(gallery, d, 1)
+    g /= np.linalg.norm(g, axis=1, keepdims=True)
+    r = np.random.default_rng(2)
+    x = torch.from_numpy(g[r.integers(0, gallery, queries)] * math.sqrt(d) + 0.3 * r.standard_normal((queries, d))).to(torch.bfloat16)
+    res = torch.from_numpy(0.1 * r.standard_normal((queries, d))).to(torch.bfloat16)
+    table = bts.mx_quantize(torch.from_numpy(g).float().cuda(), fa)
+    q, h = bts.rms_norm_mx(x.cuda(), residual=res.cuda(), fmt=fmt)
+    sim = bts.mx_product(table, q, alpha=1.0 / math.sqrt(d), floor_zero=True, dtype=torch.bfloat16).cpu().double().numpy()
+    want_h, v = norm_ref(x, res, None, 1e-6)
+    assert torch.equal(h.cpu(), want_h)
+    check_quantized(v, *host(q), fmt, d, norm_delta(d))
+    a, b = decode_ref(*host(table), fa), decode_ref(*host(q), fmt)
+    ref = np.maximum(a @ b.T / math.sqrt(d), 0)
+    assert (np.abs(sim - ref) <= product_bound(a, b, "bf16", ref, (fa, fmt))).all()
+    unit = v / np.linalg.norm(v, axis=1, keepdims=True)
+    full = bts.cosine_similarity(g.astype(np.float32), unit.astype(np.float32))
+    # a 4-bit element is off by at most 1/4 of its magnitude or an eighth of its block's unit: independent signs leave it near
+    # 0.12 / sqrt(d) * |a||b| a side; 6 of those, for both sides, and the bfloat16 output
+    assert np.abs(sim - full).max() <= 2 * 6 * 0.12 / math.sqrt(d) + 2 ** -8
+
+
+def test_two_runs_give_the_same_bits(bts):
+    a, _ = rows_of(bts, feature_rows(150, 900, 7), "e4m3")
+    b, _ = rows_of(bts, feature_rows(90, 900, 8), "e2m1")
+    x = torch.from_numpy(feature_rows(40, 900, 9)).float().cuda()
+    one, two = bts.mx_product(a, b).cpu(), bts.mx_product(a, b).cpu()
+    assert torch.equal(one, two)
+    assert torch.equal(bts.rms_norm_mx(x)[0].codes.cpu(), bts.rms_norm_mx(x)[0].codes.cpu())
+
+
+# ----------------------------------------------------------------------------------------------------------------- refusals
+
+def test_refusals(bts):
+    x = torch.ones((4, 64)).cuda()
+    q, q8 = bts.mx_quantize(x, "e2m1"), bts.mx_quantize(x, "e4m3")
+    bad = [
+        lambda: bts.mx_quantize(x, "e5m2"),
+        lambda: bts.mx_quantize(x.double()),
+        lambda: bts.mx_quantize(x[0]),
+        lambda: bts.mx_quantize(x.t()),
+        lambda: bts.mx_quantize(x[:1].expand(4, 64)),
+        lambda: bts.mx_quantize(x[:, :0]),
+        lambda: bts.mx_quantize(x, "e2m1", out=q8),
+        lambda: bts.mx_quantize(x[:3], "e2m1", out=q),
+        lambda: q.dequantize(torch.int32),
+        lambda: bts.MxRows(q.codes, q.scales, 200, "e2m1"),
+        lambda: bts.MxRows(q.codes, q.scales, 64, "e4m3"),
+        lambda: bts.MxRows(q.codes, q.scales[:3], 64, "e2m1"),
+        lambda: bts.MxRows(q.codes.t().contiguous().t(), q.scales, 64, "e2m1"),
+        lambda: bts.MxRows(q.codes, q.scales, 0, "e2m1"),
+        lambda: bts.rms_norm_mx(x, residual=x[:3]),
+        lambda: bts.rms_norm_mx(x, residual=x.half()),
+        lambda: bts.rms_norm_mx(x, weight=x[0, :63]),
+        lambda: bts.rms_norm_mx(x, weight=x[0].half()),
+        lambda: bts.rms_norm_mx(x, eps=0.0),
+        lambda: bts.rms_norm_mx(x, eps=float("nan")),
+        lambda: bts.rms_norm_mx(x, eps=float("inf")),
+        lambda: bts.rms_norm_mx(x, eps=1e-60),
+        lambda: bts.rms_norm_mx(x, fmt=None),
+        lambda: bts.rms_norm_mx(x, fmt=None, y_out=torch.empty_like(x), out=q),
+        lambda: bts.rms_norm_mx(x, fmt=None, sum_out=(s := torch.empty_like(x)), y_out=s),
+        lambda: bts.mx_product(q8, q, dtype=torch.float32),
+        lambda: bts.mx_product(q, q, dtype=torch.float64),
+        lambda: bts.mx_product(q, bts.mx_quantize(x[:, :40].contiguous())),
+        lambda: bts.mx_product(q, x),
+        lambda: bts.mx_product(q, q, out=torch.empty((4, 5)).cuda()),
+        lambda: bts.mx_product(q, q, out=torch.empty((4, 4)).cuda(), dtype=torch.float16),
+        lambda: bts.mx_product(q, q, out=torch.empty((4, 4)).cuda().t()),
+        lambda: bts.mx_row_bytes("e2m1", 0),
+    ]
+    for k, f in enumerate(bad):
+        with pytest.raises(bts.BtsError):
+            f()
+            print("accepted", k)
+
+
+def test_c_entry_refusals(bts):
+    """bad arguments at the C boundary: a status, no launch"""
+    lib, ctx = bts._lib.load(), bts._lib.default_context().handle
+    x, o = torch.ones((4, 128)).cuda(), torch.zeros((4, 128), dtype=torch.uint8).cuda()
+    s, p = torch.zeros((4, 4), dtype=torch.uint8).cuda(), lambda t, off=0: t.data_ptr() + off
+    ok = [ctx, p(x), 1, 128, 4, 128, 1, p(o), p(s), None]
+    for at, v in ((0, None), (1, None), (2, 0), (2, 7), (3, 127), (4, -1), (5, 0), (6, 2), (7, None), (7, p(o, 4)), (8, None), (8, p(s, 1)), (1, p(x, 2))):
+        assert lib.bts_mx_quantize(*(ok[:at] + [v] + ok[at + 1:])) == -1, (at, v)
+    ok = [ctx, p(o), p(s), 1, 4, 128, p(x), 1, 128, None]
+    for at, v in ((0, None), (1, None), (2, None), (3, 5), (4, -3), (5, -1), (6, None), (7, 0), (8, 100), (6, p(x, 1)), (1, p(o, 8))):
+        assert lib.bts_mx_dequantize(*(ok[:at] + [v] + ok[at + 1:])) == -1, (at, v)
+    ok = [ctx, 1, p(x), 128, None, 0, None, 4, 128, 1e-6, None, 0, None, 0, 1, p(o), p(s), None]
+    for at, v in ((0, None), (1, 0), (2, None), (3, 64), (4, p(x)), (7, -1), (8, 0), (9, 0.0), (10, p(x)), (12, p(x)), (14, 9), (15, None), (16, None), (15, p(o, 4))):
+        assert lib.bts_rms_norm(*(ok[:at] + [v] + ok[at + 1:])) == -1, (at, v)
+    ok = [ctx, p(o), p(s), 1, 4, p(o), p(s), 1, 4, 128, 1.0, 0, p(x), 3, 4, None]
+    for at, v in ((0, None), (1, None), (2, None), (3, 2), (4, -1), (5, None), (6, None), (7, -1), (8, -1), (9, 0), (12, None), (13, 0), (13, 1), (14, 3), (1, p(o, 1)), (6, p(s, 2)), (12, p(x, 1))):
+        assert lib.bts_mx_product(*(ok[:at] + [v] + ok[at + 1:])) == -1, (at, v)
+    assert (x.cpu() == 1).all() and (o.cpu() == 0).all()
+
+
+# ------------------------------------------------------------------------------------------- streams, graphs, threads (hardware)
+
+@pytest.mark.skipif("libbotsort_emu" in __import__("os").environ.get("BTS_LIB_PATH", ""), reason="needs real streams and graphs")
+class TestStreams:
+    def _pass(self, bts, x, res, table, st=None):
+        q, h = bts.rms_norm_mx(x, residual=res, fmt="e4m3")
+        return q, h, bts.mx_product(table, q, dtype=torch.bfloat16)
+
+    def _inputs(self, bts):
+        x = torch.from_numpy(feature_rows(70, 640, 1)).to(torch.bfloat16).cuda()
+        res = torch.from_numpy(feature_rows(70, 640, 2)).to(torch.bfloat16).cuda()
+        return x, res, bts.mx_quantize(torch.from_numpy(feature_rows(600, 640, 3)).float().cuda())
+
+    def test_another_stream(self, bts):
+        x, res, table = self._inputs(bts)
+        want = self._pass(bts, x, res, table)[2].cpu()
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in range(2)]
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(self._pass(bts, x, res, table)[2])
+        torch.cuda.synchronize()
+        for g in got:
+            assert torch.equal(g.cpu(), want)
+
+    def test_graph_replays(self, bts):
+        x, res, table = self._inputs(bts)
+        self._pass(bts, x, res, table)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            q, h, out = self._pass(bts, x, res, table)
+        for k in range(4):
+            nx = torch.from_numpy(feature_rows(70, 640, 50 + k)).to(torch.bfloat16).cuda()
+            x.copy_(nx)
+            graph.replay()
+            torch.cuda.synchronize()
+            eq, eh, eo = self._pass(bts, nx, res, table)
+            assert torch.equal(out.cpu(), eo.cpu()) and torch.equal(h.cpu(), eh.cpu()) and torch.equal(q.codes.cpu(), eq.codes.cpu())
