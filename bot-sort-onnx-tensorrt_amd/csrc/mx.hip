@@ -10,119 +10,143 @@ typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
-// ---- quantisation: one thread per 8 elements, four lanes per block ------------------------------------------------------------
-template <class T, int FMT, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_quantize(const T *__restrict__ x, long ldx, int n, int d, uint8_t *__restrict__ codes,
-                                                     uint8_t *__restrict__ scales) {
-    const int row8 = (int)(padded(d) / 8);                     // threads per row, a multiple of 16: a block's four lanes stay together
-    const long total = (long)n * row8;
-    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long)gridDim.x * 256) {
-        const long i = t / row8;
-        const int c = (int)(t - i * row8), k = c * 8;
+// ---- quantisation and back: one thread per 8 elements, four lanes per block, 16 lanes per 128 padded elements ------------------
+// Groups of 16 lanes walk the 128-element pieces of all rows (their number fits 32 bits: the host's check).
+template <class T, int FMT>
+__global__ __launch_bounds__(256) void k_mx_quantize(const T *__restrict__ x, long ldx, uint32_t pieces, uint32_t row_pieces, int d,
+                                                     uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
+    const int lane16 = threadIdx.x & 15;
+    for (uint32_t q = blockIdx.x * 16 + (threadIdx.x >> 4); q < pieces; q += gridDim.x * 16) {
+        const uint32_t i = q / row_pieces;
+        const int k = (int)(q - i * row_pieces) * 128 + lane16 * 8;
         float v[8] = {};
-        if (k < d) {
-            if (VEC && k + 8 <= d) load8<T, true>(x + i * ldx + k, 8, v);
-            else load8<T, false>(x + i * ldx + k, d - k, v);
-        }
+        if (k < d) load8(x + i * ldx + k, d - k, v);
         int s;
-        const uint2 q = encode_block<FMT>(v, s);
-        if (FMT == E2M1) *reinterpret_cast<uint32_t *>(codes + t * 4) = q.x;
-        else *reinterpret_cast<uint2 *>(codes + t * 8) = q;
-        if ((c & 3) == 0) scales[t >> 2] = (uint8_t)s;
+        const uint2 c = encode_block<FMT>(v, s);
+        const size_t t = (size_t)q * 16 + lane16;
+        if (FMT == E2M1) *reinterpret_cast<uint32_t *>(codes + t * 4) = c.x;
+        else *reinterpret_cast<uint2 *>(codes + t * 8) = c;
+        if ((lane16 & 3) == 0) scales[t >> 2] = (uint8_t)s;
     }
 }
 
-template <class T, int FMT, bool VEC>
-__global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, int n, int d,
-                                                       T *__restrict__ out, long ldo) {
-    const int row8 = (int)(padded(d) / 8);
-    const long total = (long)n * row8;
-    for (long t = (long)blockIdx.x * 256 + threadIdx.x; t < total; t += (long)gridDim.x * 256) {
-        const long i = t / row8;
-        const int c = (int)(t - i * row8), k = c * 8;
+template <class T, int FMT>
+__global__ __launch_bounds__(256) void k_mx_dequantize(const uint8_t *__restrict__ codes, const uint8_t *__restrict__ scales, uint32_t pieces,
+                                                       uint32_t row_pieces, int d, T *__restrict__ out, long ldo) {
+    const int lane16 = threadIdx.x & 15;
+    for (uint32_t q = blockIdx.x * 16 + (threadIdx.x >> 4); q < pieces; q += gridDim.x * 16) {
+        const uint32_t i = q / row_pieces;
+        const int k = (int)(q - i * row_pieces) * 128 + lane16 * 8;
         if (k >= d) continue;
-        const float s = scale_value(scales[t >> 2]);
-        uint2 q;
-        if (FMT == E2M1) q.x = *reinterpret_cast<const uint32_t *>(codes + t * 4);
-        else q = *reinterpret_cast<const uint2 *>(codes + t * 8);
-        float v[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const uint32_t code = FMT == E2M1 ? (q.x >> (4 * e)) & 15u : ((e < 4 ? q.x : q.y) >> (8 * (e & 3))) & 255u;
-            v[e] = decode1<FMT>(code) * s;
-        }
-        if (VEC && k + 8 <= d) store8<T, true>(out + i * ldo + k, 8, v);
-        else store8<T, false>(out + i * ldo + k, d - k, v);
+        const size_t t = (size_t)q * 16 + lane16;
+        uint2 c = {0, 0};
+        if (FMT == E2M1) c.x = *reinterpret_cast<const uint32_t *>(codes + t * 4);
+        else c = *reinterpret_cast<const uint2 *>(codes + t * 8);
+        store_words<T>(out + i * ldo + k, d - k, decode8<T, FMT>(c, scales[t >> 2]));
     }
 }
 
-// ---- root-mean-square norm: one workgroup per row -----------------------------------------------------------------------------
+// ---- root-mean-square norm -----------------------------------------------------------------------------------------------------
 template <class T> struct NormArgs {
     const T *x, *residual, *weight;
     T *sum, *y;
     long ldx, ldr, lds, ldy;
     int n, d;
-    float eps;
+    double eps;
+    int format;                          // -1: no quantised output
     uint8_t *codes, *scales;
 };
 
-template <class T, bool VEC> __device__ __forceinline__ void norm_load(const NormArgs<T> &a, long i, int k, bool from_sum, float (&h)[8]) {
-    const int have = a.d - k;
-    const bool full = VEC && have >= 8;
-    if (from_sum) {
-        if (full) load8<T, true>(a.sum + i * a.lds + k, 8, h); else load8<T, false>(a.sum + i * a.lds + k, have, h);
-        return;
-    }
-    if (full) load8<T, true>(a.x + i * a.ldx + k, 8, h); else load8<T, false>(a.x + i * a.ldx + k, have, h);
+template <class T> __device__ __forceinline__ void norm_load(const NormArgs<T> &a, long i, int k, float (&h)[8]) {
+    load8(a.x + i * a.ldx + k, a.d - k, h);
     if (!a.residual) return;
     float r[8];
-    if (full) load8<T, true>(a.residual + i * a.ldr + k, 8, r); else load8<T, false>(a.residual + i * a.ldr + k, have, r);
+    load8(a.residual + i * a.ldr + k, a.d - k, r);
     // the sum is rounded to its stored type first and normalised from there: whoever reads it back gets the same row
 #pragma unroll
-    for (int e = 0; e < 8; ++e) h[e] = to_f32(from_f32<T>(h[e] + r[e]));
+    for (int e = 0; e < 8; ++e) h[e] += r[e];
+    round8<T>(h);
+}
+// 8 squares in float32 (each product of 16-bit values is exact), the row's sum in float64: the factor of a row is common to all of its
+// elements, and a factor that is off by a few roundings turns that many codes at the borders between two values
+__device__ __forceinline__ double squares(const float (&h)[8]) {
+    return (double)(((h[0] * h[0] + h[1] * h[1]) + (h[2] * h[2] + h[3] * h[3])) + ((h[4] * h[4] + h[5] * h[5]) + (h[6] * h[6] + h[7] * h[7])));
+}
+// the normalised piece at column k: to y, and as codes (whole blocks: a block's four lanes come together)
+template <class T> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, float inv, float (&h)[8]) {
+    if (k < a.d) {
+        if (a.weight) {
+            float w[8];
+            load8(a.weight + k, a.d - k, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] *= w[e];             // (exact for 16-bit types: one rounding, that of the factor, follows)
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) h[e] = k + e < a.d ? h[e] * inv : 0.0f;
+        if (a.y) store8(a.y + i * a.ldy + k, a.d - k, h);
+    }
+    if (a.format < 0) return;
+    int s;
+    const size_t t = ((size_t)i * width + k) / 8;
+    if (a.format == E2M1) *reinterpret_cast<uint32_t *>(a.codes + t * 4) = encode_block<E2M1>(h, s).x;
+    else *reinterpret_cast<uint2 *>(a.codes + t * 8) = encode_block<E4M3>(h, s);
+    if ((threadIdx.x & 3) == 0) a.scales[t >> 2] = (uint8_t)s;
 }
 
-// FMT: E2M1, E4M3, or -1 (no quantised output)
-template <class T, int FMT, bool VEC>
+// TPR threads per row, CH pieces of 8 elements a thread: the row stays in registers between the sum and the output, so x and residual
+// are read once.  CH = 0: rows beyond 8192 elements, in two passes; the second reads the stored sum, or x and residual again.
+// One pass over memory bounds it (32768 x 4096 bfloat16 with residual and weight: 0.94 GB).
+template <class T, int TPR, int CH>
 __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
-    __shared__ float part[4];
-    const long i = blockIdx.x;
-    const int width = (int)padded(a.d);
-    float ss = 0.0f;
-    for (int k = threadIdx.x * 8; k < a.d; k += 2048) {
-        float h[8];
-        norm_load<T, VEC>(a, i, k, false, h);
-        if (a.sum) { if (VEC && k + 8 <= a.d) store8<T, true>(a.sum + i * a.lds + k, 8, h); else store8<T, false>(a.sum + i * a.lds + k, a.d - k, h); }
+    __shared__ double part[4];
+    const long i = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const int width = (int)padded(a.d), first = (threadIdx.x % TPR) * 8;
+    if (TPR == 64 && i >= a.n) return;
+    float h[CH > 0 ? CH : 1][8];
+    double ss = 0.0;
+    if (CH > 0) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(h[e], h[e], ss);
+        for (int c = 0; c < CH; ++c) {
+            const int k = first + c * TPR * 8;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[c][e] = 0.0f;
+            if (k < a.d) norm_load(a, i, k, h[c]);
+        }
+#pragma unroll
+        for (int c = 0; c < CH; ++c) {
+            const int k = first + c * TPR * 8;
+            if (a.sum && k < a.d) store8(a.sum + i * a.lds + k, a.d - k, h[c]);
+            ss += squares(h[c]);
+        }
+    } else {
+        for (int k = first; k < a.d; k += TPR * 8) {
+            norm_load(a, i, k, h[0]);
+            if (a.sum) store8(a.sum + i * a.lds + k, a.d - k, h[0]);
+            ss += squares(h[0]);
+        }
     }
 #pragma unroll
     for (int m = 32; m; m >>= 1) ss += __shfl_xor(ss, m);
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
-    __syncthreads();
-    ss = (part[0] + part[1]) + (part[2] + part[3]);
-    const float inv = 1.0f / sqrtf(ss / (float)a.d + a.eps);
-    for (int k = threadIdx.x * 8; k < width; k += 2048) {
-        float h[8] = {};
-        if (k < a.d) {
-            norm_load<T, VEC>(a, i, k, a.sum != nullptr, h);
-            float w[8];
-            if (a.weight) { if (VEC && k + 8 <= a.d) load8<T, true>(a.weight + k, 8, w); else load8<T, false>(a.weight + k, a.d - k, w); }
+    if (TPR == 256) {
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = ss;
+        __syncthreads();
+        ss = (part[0] + part[1]) + (part[2] + part[3]);
+    }
+    const float inv = (float)(1.0 / sqrt(ss / (double)a.d + a.eps));
+    if (CH > 0) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] = a.weight ? h[e] * inv * w[e] : h[e] * inv;
-            if (!(VEC && k + 8 <= a.d)) {                       // behind the end: zeros, whatever inv is
-#pragma unroll
-                for (int e = 0; e < 8; ++e) h[e] = k + e < a.d ? h[e] : 0.0f;
-            }
-            if (a.y) { if (VEC && k + 8 <= a.d) store8<T, true>(a.y + i * a.ldy + k, 8, h); else store8<T, false>(a.y + i * a.ldy + k, a.d - k, h); }
+        for (int c = 0; c < CH; ++c) {
+            const int k = first + c * TPR * 8;
+            if (k < width) norm_emit(a, i, k, width, inv, h[c]);
         }
-        if (FMT >= 0) {
-            int s;
-            const uint2 q = encode_block<FMT == E2M1 ? E2M1 : E4M3>(h, s);
-            const long t = (i * width + k) / 8;
-            if (FMT == E2M1) *reinterpret_cast<uint32_t *>(a.codes + t * 4) = q.x;
-            else *reinterpret_cast<uint2 *>(a.codes + t * 8) = q;
-            if ((threadIdx.x & 3) == 0) a.scales[t >> 2] = (uint8_t)s;
+    } else {
+        for (int k = first; k < width; k += TPR * 8) {
+            if (k >= a.d) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) h[0][e] = 0.0f;
+            } else if (a.sum) load8(a.sum + i * a.lds + k, a.d - k, h[0]);
+            else norm_load(a, i, k, h[0]);
+            norm_emit(a, i, k, width, inv, h[0]);
         }
     }
 }
@@ -140,7 +164,7 @@ struct ProductArgs {
     void *out;
     int out_dtype;
     long ld;
-    int out_vec;                         // 4 consecutive outputs may be stored as one vector (alignment of out and ld)
+    int out_vec;                         // rows may be stored 16 bytes at a time (alignment of out and ld)
 };
 
 template <int FMT> __device__ __forceinline__ v8i load_fragment(const uint8_t *row, int step, int g) {
@@ -156,7 +180,29 @@ template <int FMT> __device__ __forceinline__ v8i load_fragment(const uint8_t *r
     }
     return f;
 }
-template <int FMT> constexpr int mfma_code() { return FMT == E2M1 ? 4 : 0; }      // the instruction's format selectors
+template <int FMT> constexpr int MFMA_CODE = FMT == E2M1 ? 4 : 0;      // the instruction's format selectors
+
+// acc += B fragment x A fragment, scale byte OB of sb and OA of sa
+template <int FA, int FB, int OA, int OB> __device__ __forceinline__ v4f mma(v8i fb, v8i fa, v4f acc, int sb, int sa) {
+    return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb, fa, acc, (MFMA_CODE<FB>), (MFMA_CODE<FA>), OB, sb, OA, sa);
+}
+// (the byte selectors are immediates: the cases fold away in unrolled loops)
+template <int FA, int FB, int OA> __device__ __forceinline__ v4f mma_b(v8i fb, v8i fa, v4f acc, int sb, int ob, int sa) {
+    switch (ob & 3) {
+        case 0: return mma<FA, FB, OA, 0>(fb, fa, acc, sb, sa);
+        case 1: return mma<FA, FB, OA, 1>(fb, fa, acc, sb, sa);
+        case 2: return mma<FA, FB, OA, 2>(fb, fa, acc, sb, sa);
+        default: return mma<FA, FB, OA, 3>(fb, fa, acc, sb, sa);
+    }
+}
+template <int FA, int FB> __device__ __forceinline__ v4f mma_bytes(v8i fb, v8i fa, v4f acc, int sb, int ob, int sa, int oa) {
+    switch (oa & 3) {
+        case 0: return mma_b<FA, FB, 0>(fb, fa, acc, sb, ob, sa);
+        case 1: return mma_b<FA, FB, 1>(fb, fa, acc, sb, ob, sa);
+        case 2: return mma_b<FA, FB, 2>(fb, fa, acc, sb, ob, sa);
+        default: return mma_b<FA, FB, 3>(fb, fa, acc, sb, ob, sa);
+    }
+}
 
 template <class T> __device__ __forceinline__ void store_out4(T *p, int have, bool vec, const float (&v)[4]) {
     if (vec && have >= 4) {
@@ -169,15 +215,18 @@ template <class T> __device__ __forceinline__ void store_out4(T *p, int have, bo
         for (int e = 0; e < 4; ++e) if (e < have) p[e] = from_f32<T>(v[e]);
     }
 }
-// four consecutive columns j .. j + 3 of row i
-__device__ __forceinline__ void epilogue4(const ProductArgs &p, long i, int j, v4f acc) {
-    if (i >= p.n || j >= p.m) return;
-    float v[4];
+__device__ __forceinline__ void finish(const ProductArgs &p, v4f acc, float (&v)[4]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
         v[e] = acc[e] * p.alpha;
         if (p.floor_zero) v[e] = v[e] < 0.0f ? 0.0f : v[e];       // (a NaN stays one)
     }
+}
+// four consecutive columns j .. j + 3 of row i
+__device__ __forceinline__ void epilogue4(const ProductArgs &p, long i, int j, v4f acc) {
+    if (i >= p.n || j >= p.m) return;
+    float v[4];
+    finish(p, acc, v);
     const long at = i * p.ld + j;
     const int have = p.m - j;
     if (p.out_dtype == BTS_F32) store_out4(static_cast<float *>(p.out) + at, have, p.out_vec, v);
@@ -185,65 +234,269 @@ __device__ __forceinline__ void epilogue4(const ProductArgs &p, long i, int j, v
     else store_out4(static_cast<bf16 *>(p.out) + at, have, p.out_vec, v);
 }
 
-// A workgroup of KW wavefronts computes a (16 RT) x (16 CT) tile; each wavefront takes a contiguous part of the row, straight from
-// memory to registers, and the parts are added through LDS in a fixed order.
-template <int FA, int FB, int RT, int CT, int KW>
-__global__ __launch_bounds__(64 * KW) void k_mx_direct(ProductArgs p) {
-    __shared__ v4f part[KW > 1 ? KW - 1 : 1][RT * CT][64];
-    const int tiles_n = (p.m + 16 * CT - 1) / (16 * CT);
-    const int ti = (int)(blockIdx.x / (unsigned)tiles_n), tj = (int)(blockIdx.x % (unsigned)tiles_n);
+// A workgroup of 4 wavefronts computes one 16 x 16 tile straight from memory; each wavefront takes a quarter of the row, and the parts are
+// added through LDS in a fixed order.  For few tiles, where the length of a row is what takes time (1 x 2000 x 2048: 3.6 us against 5.4
+// with LDS tiles; 1 x 300 x 8192: 7.4 against 12.4), and for sizes beyond the tiles' 32-bit offsets.
+template <int FA, int FB>
+__global__ __launch_bounds__(256) void k_mx_direct(ProductArgs p) {
+    __shared__ v4f part[3][64];
+    const long tiles_n = ((long)p.m + 15) / 16, ti = blockIdx.x / tiles_n, tj = blockIdx.x % tiles_n;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
-    const uint8_t *ac[RT], *as[RT], *bc[CT], *bs[CT];
-    const long step_a = FA == E2M1 ? 64 : 128, step_b = FB == E2M1 ? 64 : 128;
-#pragma unroll
-    for (int u = 0; u < RT; ++u) {                                 // rows behind the last one read the last one; never stored
-        const long i = min((long)ti * 16 * RT + 16 * u + r, (long)p.n - 1);
-        ac[u] = p.a_codes + i * p.steps * step_a; as[u] = p.a_scales + i * p.steps * 4 + g;
+    const long i = min(ti * 16 + r, (long)p.n - 1), j = min(tj * 16 + r, (long)p.m - 1);      // (rows behind the last one read it; never stored)
+    const uint8_t *ac = p.a_codes + i * p.steps * (FA == E2M1 ? 64 : 128), *as = p.a_scales + i * p.steps * 4 + g;
+    const uint8_t *bc = p.b_codes + j * p.steps * (FB == E2M1 ? 64 : 128), *bs = p.b_scales + j * p.steps * 4 + g;
+    const int per = (p.steps + 3) / 4, s0 = wave * per, s1 = min(p.steps, s0 + per);
+    v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 2
+    for (int s = s0; s < s1; ++s)
+        acc = mma<FA, FB, 0, 0>(load_fragment<FB>(bc, s, g), load_fragment<FA>(ac, s, g), acc, bs[(long)s * 4], as[(long)s * 4]);
+    if (wave > 0) part[wave - 1][lane] = acc;
+    __syncthreads();
+    if (wave > 0) return;
+    acc = ((acc + part[0][lane]) + part[1][lane]) + part[2][lane];
+    epilogue4(p, ti * 16 + r, (int)tj * 16 + 4 * g, acc);
+}
+
+// XCD-aware order of the tiles: the 8 XCDs have an L2 each and take workgroups in turn, so every XCD gets a contiguous run of tiles, and a
+// run goes down groups of 8 tile rows, column by column: the tiles that are in flight together share their A and B rows.
+__device__ __forceinline__ void tile_of(int bid, int tiles_m, int tiles_n, int &tm, int &tn) {
+    const int all = tiles_m * tiles_n, q = all / 8, rest = all % 8, xcd = bid % 8, slot = bid / 8;
+    const int v = (xcd < rest ? xcd * (q + 1) : rest * (q + 1) + (xcd - rest) * q) + slot;
+    const int group = v / (8 * tiles_n), first = group * 8, rows = min(8, tiles_m - first), in = v - group * 8 * tiles_n;
+    tm = first + in % rows;
+    tn = in / rows;
+}
+
+// The rows of one tile as a bounded buffer: what lies behind the last row reads as zeros, so no load needs a clamped address.
+struct TileRows {
+    __amdgpu_buffer_rsrc_t rsrc;
+    __device__ __forceinline__ TileRows(const uint8_t *base, int row, int rows, int tile, int stride) {
+        rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + (long)row * stride), 0, min(tile, rows - row) * stride, 0x00020000);
     }
+    __device__ __forceinline__ v4i load16(int at) const { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)); }
+    __device__ __forceinline__ uint32_t load4(int at) const { return __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0); }
+};
+
+// One operand of a stage: ROWS rows of SK instruction depths, moved by THREADS threads.  A row of a stage is C 16-byte chunks; chunk c of
+// row r lies at c ^ swizzle(r), so that the 16 lanes that an LDS read serves at a time -- 16 rows of one chunk, or 8 rows of each of two
+// neighbouring chunks -- are in 16 different 16-byte bank groups (no bank conflict counted; 4 cycles a read with rows / 4 in the
+// 64-byte rows' swizzle instead of its negative).
+template <int FMT, int ROWS, int THREADS, int SK> struct Operand {
+    static constexpr int S1 = FMT == E2M1 ? 64 : 128, S = SK * S1;                // bytes a row: an instruction depth, a stage
+    static constexpr int C = S / 16, STEP = THREADS / C;                         // chunks a row; rows between a thread's chunks
+    static constexpr int MOVES = ROWS * C < THREADS ? 1 : ROWS * C / THREADS;    // chunks a thread moves (at most, if there are fewer than threads)
+    static constexpr int PERIOD = STEP % 16 == 0 ? 1 : 16 / STEP;                // moves after which the swizzle repeats
+    static constexpr int BYTES = ROWS * S;
+    static_assert((MOVES * THREADS == ROWS * C || MOVES == 1) && MOVES % PERIOD == 0, "even staging");
+    static __device__ __forceinline__ int swizzle(int row) { return (C >= 16 ? row : C == 8 ? row / 2 : -(row / 4)) & (C >= 16 ? 15 : C - 1); }
+    int from, to[PERIOD], frag[SK][S1 / 64];
+    struct Regs { v4i chunk[MOVES]; };
+    __device__ __forceinline__ void init(int tid, int first_row, int r, int g, int stride) {
+        const int row = tid / C, c = tid % C;
+        from = row * stride + c * 16;
 #pragma unroll
-    for (int u = 0; u < CT; ++u) {
-        const long j = min((long)tj * 16 * CT + 16 * u + r, (long)p.m - 1);
-        bc[u] = p.b_codes + j * p.steps * step_b; bs[u] = p.b_scales + j * p.steps * 4 + g;
+        for (int q = 0; q < PERIOD; ++q) to[q] = (row + q * STEP) * S + (c ^ swizzle(row + q * STEP)) * 16;
+#pragma unroll
+        for (int k = 0; k < SK; ++k)
+#pragma unroll
+            for (int h = 0; h < S1 / 64; ++h) frag[k][h] = (first_row + r) * S + ((k * (S1 / 16) + 4 * h + g) ^ swizzle(r)) * 16;
     }
+    __device__ __forceinline__ void load(Regs &x, const TileRows &rows, int stage, int stride) const {
+#pragma unroll
+        for (int q = 0; q < MOVES; ++q) x.chunk[q] = rows.load16(from + q * STEP * stride + stage * S);
+    }
+    __device__ __forceinline__ void store(const Regs &x, uint8_t *image) const {
+#pragma unroll
+        for (int q = 0; q < MOVES; ++q)
+            if (MOVES * THREADS == ROWS * C || to[0] < BYTES) *reinterpret_cast<v4i *>(image + to[q % PERIOD] + (q / PERIOD) * PERIOD * STEP * S) = x.chunk[q];
+    }
+    // the fragment of the 16 rows `u` times 16 behind the wavefront's first one, depth k of the stage
+    __device__ __forceinline__ v8i fragment(const uint8_t *image, int u, int k) const {
+        v8i f = {};
+        const v4i lo = *reinterpret_cast<const v4i *>(image + frag[k][0] + u * S * 16);
+        f[0] = lo[0]; f[1] = lo[1]; f[2] = lo[2]; f[3] = lo[3];
+        if (S1 == 128) {
+            const v4i hi = *reinterpret_cast<const v4i *>(image + frag[k][S1 / 64 - 1] + u * S * 16);
+            f[4] = hi[0]; f[5] = hi[1]; f[6] = hi[2]; f[7] = hi[3];
+        }
+        return f;
+    }
+};
+
+// A wavefront's (16 RT) x (16 CT) results leave through its own 2 KB of LDS, 16 rows of 128 bytes at a time, so that whole 128-byte lines are
+// stored (16 rows of 8 or 16 bytes a lane straight from the accumulators cost 1.5 us more a round of 256 x 256 bfloat16 tiles).  Chunk c
+// of row r lies at c ^ r.  Rows that cannot be stored 16 bytes at a time go element by element, neighbours in neighbouring lanes.
+template <class T, int RT, int CT>
+__device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc)[RT][CT], uint8_t *room, int i0, int j0, int lane) {
+    constexpr int FRAGS = 8 / (int)sizeof(T) < CT ? 8 / (int)sizeof(T) : CT, COLS = FRAGS * 16, ROWB = COLS * (int)sizeof(T), CHUNKS = ROWB / 16;
+    constexpr int ACROSS = 64 / CHUNKS < 16 ? 64 / CHUNKS : 16;                    // rows a store
+    static_assert(CT % FRAGS == 0, "whole passes");
+    const int r = lane & 15, g = lane >> 4, rows = p.n - i0, cols = p.m - j0, ld = (int)p.ld * (int)sizeof(T);      // (bytes; the host's check)
+    uint8_t *const out = reinterpret_cast<uint8_t *>(static_cast<T *>(p.out) + (i0 * p.ld + j0));                   // the same in all lanes
+    const int row8 = lane / CHUNKS, at8 = row8 * ld + (lane % CHUNKS) * 16;
+#pragma unroll
+    for (int u = 0; u < RT; ++u)
+#pragma unroll
+        for (int w0 = 0; w0 < CT; w0 += FRAGS) {
+#pragma unroll
+            for (int w = 0; w < FRAGS; ++w) {
+                float v[4];
+                finish(p, acc[u][w0 + w], v);
+                const int at = (w * 16 + 4 * g) * (int)sizeof(T);
+                store_out4(reinterpret_cast<T *>(room + r * ROWB + ((at / 16) ^ (r & (CHUNKS - 1))) * 16 + at % 16), 4, true, v);
+            }
+            __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if (p.out_vec && w0 * 16 + COLS <= cols) {
+#pragma unroll
+                for (int q = 0; q < 16 / ACROSS; ++q) {
+                    const int row = q * ACROSS + row8;
+                    if (64 / CHUNKS > 16 && row >= 16) break;
+                    const v4i x = *reinterpret_cast<const v4i *>(room + row * ROWB + ((lane % CHUNKS) ^ (row & (CHUNKS - 1))) * 16);
+                    if (u * 16 + row < rows) *reinterpret_cast<v4i *>(out + (uint32_t)(at8 + (u * 16 + q * ACROSS) * ld + w0 * 16 * (int)sizeof(T))) = x;
+                }
+            } else {
+#pragma unroll 4
+                for (int q = 0; q < 16 * COLS / 64; ++q) {
+                    const int row = q * (64 / COLS) + lane / COLS, col = lane % COLS, at = col * (int)sizeof(T);
+                    const T x = *reinterpret_cast<const T *>(room + row * ROWB + ((at / 16) ^ (row & (CHUNKS - 1))) * 16 + at % 16);
+                    if (u * 16 + row < rows && w0 * 16 + col < cols) *reinterpret_cast<T *>(out + (uint32_t)((u * 16 + row) * ld + (w0 * 16 + col) * (int)sizeof(T))) = x;
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+// A workgroup of WM x WN wavefronts computes a TM x TN tile in stages of SK instruction depths of 128 elements.  A stage's codes and scale
+// bytes go from memory through registers to one of two LDS images while the other is multiplied; the loads of AHEAD stages are in flight.
+// (Fragments straight from memory would be 16 rows x 64 bytes a load with the lanes of a row 16 apart: a quarter of the load path's rate.)
+// With 8 wavefronts (two a SIMD) the second four run one phase behind the first: while one of a SIMD's two wavefronts multiplies, the
+// other fetches its fragments, stores the next stage and issues the loads of the one after; barriers keep the two in step.  With 4
+// wavefronts a stage has one barrier, and the workgroups of a CU take turns.
+template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD>
+__global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
+    constexpr int THREADS = 64 * WM * WN, RT = TM / WM / 16, CT = TN / WN / 16;
+    constexpr bool PHASED = WM * WN == 8;
+    typedef Operand<FA, TM, THREADS, SK> OpA;
+    typedef Operand<FB, TN, THREADS, SK> OpB;
+    static_assert((RT % 4 == 0 || TM <= 64) && (CT % 4 == 0 || TN <= 64), "scale bytes come four fragments to a word");
+    constexpr int GA = (TM + 63) / 64, GB = (TN + 63) / 64;  // groups of 64 rows = four fragments
+    constexpr int WORDS = (TM + TN) * SK, SMOVES = (WORDS + THREADS - 1) / THREADS;
+    constexpr int B_AT = 2 * OpA::BYTES, IMAGES = B_AT + 2 * OpB::BYTES, ROOM = WM * WN * 2048;      // A's two images, then B's
+    __shared__ __attribute__((aligned(1024))) uint8_t image[IMAGES > ROOM ? IMAGES : ROOM];
+    // scale bytes: [group][lane group][row of a fragment][fragment], so that a lane's four are one word
+    __shared__ __attribute__((aligned(16))) uint8_t lscale[2][SK][GA + GB][4][16][4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int wm = wave / WN, wn = wave % WN;
+    const int first_a = 8 * (wm * RT % 4), first_b = 8 * (wn * CT % 4);      // where a wavefront's fragments begin in their group's words
+    int tm, tn;
+    tile_of(blockIdx.x, (p.n + TM - 1) / TM, (p.m + TN - 1) / TN, tm, tn);
+
+    const int stride_a = p.steps * OpA::S1, stride_b = p.steps * OpB::S1, stride_s = p.steps * 4, stages = (p.steps + SK - 1) / SK;
+    const TileRows ga(p.a_codes, tm * TM, p.n, TM, stride_a), gb(p.b_codes, tn * TN, p.m, TN, stride_b);
+    const TileRows gsa(p.a_scales, tm * TM, p.n, TM, stride_s), gsb(p.b_scales, tn * TN, p.m, TN, stride_s);
+    OpA a;
+    OpB b;
+    a.init(tid, wm * RT * 16, r, g, stride_a);
+    b.init(tid, wn * CT * 16, r, g, stride_b);
+    // (depths behind the row's end load the next row's beginning, or zeros; they are not multiplied)
+    struct Stage { typename OpA::Regs a; typename OpB::Regs b; uint32_t scale[SMOVES]; };
+    const auto load = [&](Stage &st, int stage) {
+        if (stage >= stages) return;
+        a.load(st.a, ga, stage, stride_a);
+        b.load(st.b, gb, stage, stride_b);
+#pragma unroll
+        for (int q = 0; q < SMOVES; ++q) {
+            const int word = tid + q * THREADS, row = word / SK, k = word % SK, at = (stage * SK + k) * 4;
+            if (row < TM) st.scale[q] = gsa.load4(row * stride_s + at);
+            else if (row < TM + TN) st.scale[q] = gsb.load4((row - TM) * stride_s + at);
+        }
+    };
+    const auto store = [&](const Stage &st, int stage) {
+        if (stage >= stages) return;
+        const int buf = stage & 1;
+        a.store(st.a, image + buf * OpA::BYTES);
+        b.store(st.b, image + B_AT + buf * OpB::BYTES);
+#pragma unroll
+        for (int q = 0; q < SMOVES; ++q) {
+            const int word = tid + q * THREADS, k = word % SK, row = word / SK < TM ? word / SK : word / SK - TM, base = word / SK < TM ? 0 : GA;
+            if (word < WORDS) {
+                uint8_t *to = &lscale[buf][k][base + (row >> 6)][0][row & 15][(row >> 4) & 3];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) to[64 * e] = (uint8_t)(st.scale[q] >> (8 * e));
+            }
+        }
+    };
     v4f acc[RT][CT];
 #pragma unroll
     for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int w = 0; w < CT; ++w) acc[u][w] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    const int per = (p.steps + KW - 1) / KW, s0 = wave * per, s1 = min(p.steps, s0 + per);
-    for (int s = s0; s < s1; ++s) {
-        v8i fa[RT], fb[CT];
-        int sa[RT], sb[CT];
+    // stage t, the next one in `next`
+    const auto step = [&](int t, Stage &next) {
+        const int buf = t & 1;
 #pragma unroll
-        for (int u = 0; u < RT; ++u) { fa[u] = load_fragment<FA>(ac[u], s, g); sa[u] = as[u][(long)s * 4]; }
+        for (int k = 0; k < SK; ++k) {
+            if (k > 0 && t * SK + k >= p.steps) break;
+            v8i fa[RT], fb[CT];
+            int sa[(RT + 3) / 4], sb[(CT + 3) / 4];
 #pragma unroll
-        for (int w = 0; w < CT; ++w) { fb[w] = load_fragment<FB>(bc[w], s, g); sb[w] = bs[w][(long)s * 4]; }
+            for (int u = 0; u < RT; ++u) fa[u] = a.fragment(image + buf * OpA::BYTES, u, k);
 #pragma unroll
-        for (int u = 0; u < RT; ++u)
+            for (int w = 0; w < CT; ++w) fb[w] = b.fragment(image + B_AT + buf * OpB::BYTES, w, k);
+#pragma unroll
+            for (int q = 0; q < (RT + 3) / 4; ++q) sa[q] = *reinterpret_cast<const int *>(&lscale[buf][k][wm * RT / 4 + q][g][r][0]) >> first_a;
+#pragma unroll
+            for (int q = 0; q < (CT + 3) / 4; ++q) sb[q] = *reinterpret_cast<const int *>(&lscale[buf][k][GA + wn * CT / 4 + q][g][r][0]) >> first_b;
+            if (PHASED) {
+                if (k == 0) {
+                    store(next, t + 1);
+                    load(next, t + 1 + AHEAD);
+                }
+                __builtin_amdgcn_sched_barrier(0);
+                __syncthreads();
+                __builtin_amdgcn_s_setprio(1);
+            }
 #pragma unroll
             for (int w = 0; w < CT; ++w)
-                acc[u][w] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(fb[w], fa[u], acc[u][w], mfma_code<FB>(), mfma_code<FA>(), 0, sb[w], 0, sa[u]);
-    }
-    if (KW > 1) {
-        if (wave > 0) {
 #pragma unroll
-            for (int u = 0; u < RT; ++u)
-#pragma unroll
-                for (int w = 0; w < CT; ++w) part[wave - 1][u * CT + w][lane] = acc[u][w];
+                for (int u = 0; u < RT; ++u)
+                    acc[u][w] = mma_bytes<FA, FB>(fb[w], fa[u], acc[u][w], sb[w / 4], w, sa[u / 4], u);
+            if (PHASED) {
+                __builtin_amdgcn_s_setprio(0);
+                __builtin_amdgcn_sched_barrier(0);
+                __syncthreads();
+            }
         }
-        __syncthreads();
-        if (wave > 0) return;
-#pragma unroll
-        for (int q = 0; q < KW - 1; ++q)
-#pragma unroll
-            for (int u = 0; u < RT; ++u)
-#pragma unroll
-                for (int w = 0; w < CT; ++w) acc[u][w] += part[q][u * CT + w][lane];
+        if (!PHASED) {
+            store(next, t + 1);
+            load(next, t + 1 + AHEAD);
+            __syncthreads();
+        }
+    };
+    Stage odd, even;                                         // (AHEAD 1: every stage goes through `odd`)
+    load(odd, 0);
+    if (AHEAD == 2) load(even, 1);
+    store(odd, 0);
+    load(odd, AHEAD);
+    __syncthreads();
+    if (PHASED && wave >= 4) __syncthreads();
+    if (AHEAD == 1) {
+        for (int t = 0; t < stages; ++t) step(t, odd);
+    } else {
+        for (int t = 0; t < stages; t += 2) {
+            step(t, even);
+            if (t + 1 < stages) step(t + 1, odd);
+        }
     }
-#pragma unroll
-    for (int u = 0; u < RT; ++u)
-#pragma unroll
-        for (int w = 0; w < CT; ++w) epilogue4(p, (long)ti * 16 * RT + 16 * u + r, tj * 16 * CT + 16 * w + 4 * g, acc[u][w]);
+    if (PHASED && wave < 4) __syncthreads();
+    uint8_t *room = image + wave * 2048;
+    const int i0 = tm * TM + wm * RT * 16, j0 = tn * TN + wn * CT * 16;
+    if (i0 >= p.n || j0 >= p.m) return;                      // (all of this wavefront's rows or columns lie behind the last one)
+    if (p.out_dtype == BTS_F32) write_tile<float, RT, CT>(p, acc, room, i0, j0, lane);
+    else if (p.out_dtype == BTS_F16) write_tile<_Float16, RT, CT>(p, acc, room, i0, j0, lane);
+    else write_tile<bf16, RT, CT>(p, acc, room, i0, j0, lane);
 }
 
 // ---- host side ----------------------------------------------------------------------------------------------------------------
@@ -251,62 +504,71 @@ bool known_format(int f) { return f == BTS_MX_E2M1 || f == BTS_MX_E4M3; }
 bool known_dtype(int t) { return t == BTS_F32 || t == BTS_F16 || t == BTS_BF16; }
 size_t dtype_bytes(int t) { return t == BTS_F32 ? 4 : 2; }
 bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
-int row_grid(const bts_context *ctx, int n, int d) {           // workgroups of 256 threads, one thread per 8 elements
-    const long blocks = ((long)n * (padded(d) / 8) + 255) / 256, most = (long)ctx->n_cu * 64;
-    return (int)(blocks < most ? blocks : most);
+constexpr long MOST_PIECES = 0xffffffffl - (1 << 24);          // 128-element pieces a call takes (the grid's stride is added in 32 bits)
+long pieces(int n, int d) { return (long)n * (padded(d) / MX_ROW); }
+dim3 piece_grid(const bts_context *ctx, long pieces) {
+    const long blocks = (pieces + 15) / 16, most = (long)ctx->n_cu * 64;
+    return dim3((unsigned)(blocks < most ? blocks : most));
 }
 
-template <class T> int quantize(bts_context *ctx, const T *x, int ldx, int n, int d, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
-    const bool vec = aligned(x, 16) && (size_t)ldx * sizeof(T) % 16 == 0;
-    const dim3 grid(row_grid(ctx, n, d)), block(256);
-    if (format == E2M1) {
-        if (vec) hipLaunchKernelGGL((k_mx_quantize<T, E2M1, true>), grid, block, 0, st, x, (long)ldx, n, d, codes, scales);
-        else hipLaunchKernelGGL((k_mx_quantize<T, E2M1, false>), grid, block, 0, st, x, (long)ldx, n, d, codes, scales);
-    } else {
-        if (vec) hipLaunchKernelGGL((k_mx_quantize<T, E4M3, true>), grid, block, 0, st, x, (long)ldx, n, d, codes, scales);
-        else hipLaunchKernelGGL((k_mx_quantize<T, E4M3, false>), grid, block, 0, st, x, (long)ldx, n, d, codes, scales);
-    }
-    BTS_LAUNCH_CHECK();
-    return BTS_OK;
+template <class T> void quantize(bts_context *ctx, const void *x, int ldx, int n, int d, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
+    const uint32_t all = (uint32_t)pieces(n, d), row = (uint32_t)(padded(d) / MX_ROW);
+    const T *const xs = static_cast<const T *>(x);
+    if (format == E2M1) hipLaunchKernelGGL((k_mx_quantize<T, E2M1>), piece_grid(ctx, all), dim3(256), 0, st, xs, (long)ldx, all, row, d, codes, scales);
+    else hipLaunchKernelGGL((k_mx_quantize<T, E4M3>), piece_grid(ctx, all), dim3(256), 0, st, xs, (long)ldx, all, row, d, codes, scales);
+}
+template <class T> void dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *scales, int format, int n, int d, void *out, int ldo, hipStream_t st) {
+    const uint32_t all = (uint32_t)pieces(n, d), row = (uint32_t)(padded(d) / MX_ROW);
+    T *const to = static_cast<T *>(out);
+    if (format == E2M1) hipLaunchKernelGGL((k_mx_dequantize<T, E2M1>), piece_grid(ctx, all), dim3(256), 0, st, codes, scales, all, row, d, to, (long)ldo);
+    else hipLaunchKernelGGL((k_mx_dequantize<T, E4M3>), piece_grid(ctx, all), dim3(256), 0, st, codes, scales, all, row, d, to, (long)ldo);
 }
 
-template <class T> int dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *scales, int format, int n, int d, T *out, int ldo, hipStream_t st) {
-    const bool vec = aligned(out, 16) && (size_t)ldo * sizeof(T) % 16 == 0;
-    const dim3 grid(row_grid(ctx, n, d)), block(256);
-    if (format == E2M1) {
-        if (vec) hipLaunchKernelGGL((k_mx_dequantize<T, E2M1, true>), grid, block, 0, st, codes, scales, n, d, out, (long)ldo);
-        else hipLaunchKernelGGL((k_mx_dequantize<T, E2M1, false>), grid, block, 0, st, codes, scales, n, d, out, (long)ldo);
-    } else {
-        if (vec) hipLaunchKernelGGL((k_mx_dequantize<T, E4M3, true>), grid, block, 0, st, codes, scales, n, d, out, (long)ldo);
-        else hipLaunchKernelGGL((k_mx_dequantize<T, E4M3, false>), grid, block, 0, st, codes, scales, n, d, out, (long)ldo);
-    }
-    BTS_LAUNCH_CHECK();
-    return BTS_OK;
+template <class T, int TPR, int CH> void rms_norm_launch(const NormArgs<T> &a, hipStream_t st) {
+    const int rows = 256 / TPR;
+    hipLaunchKernelGGL((k_rms_norm<T, TPR, CH>), dim3((unsigned)(((long)a.n + rows - 1) / rows)), dim3(256), 0, st, a);
 }
-
-template <class T, int FMT> void rms_norm_launch(const NormArgs<T> &a, bool vec, hipStream_t st) {
-    if (vec) hipLaunchKernelGGL((k_rms_norm<T, FMT, true>), dim3(a.n), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_rms_norm<T, FMT, false>), dim3(a.n), dim3(256), 0, st, a);
-}
-template <class T> int rms_norm(const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d, float eps,
-                                void *sum, int lds, void *y, int ldy, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
+template <class T> void rms_norm(const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d, double eps,
+                                 void *sum, int lds, void *y, int ldy, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
     NormArgs<T> a;
     a.x = static_cast<const T *>(x); a.residual = static_cast<const T *>(residual); a.weight = static_cast<const T *>(weight);
     a.sum = static_cast<T *>(sum); a.y = static_cast<T *>(y);
-    a.ldx = ldx; a.ldr = ldr; a.lds = lds; a.ldy = ldy; a.n = n; a.d = d; a.eps = eps; a.codes = codes; a.scales = scales;
-    const auto fits = [](const void *p, long ld) { return !p || (aligned(p, 16) && (size_t)ld * sizeof(T) % 16 == 0); };
-    const bool vec = fits(x, ldx) && fits(residual, ldr) && fits(weight, 0) && fits(sum, lds) && fits(y, ldy);
-    if (format == E2M1) rms_norm_launch<T, E2M1>(a, vec, st);
-    else if (format == E4M3) rms_norm_launch<T, E4M3>(a, vec, st);
-    else rms_norm_launch<T, -1>(a, vec, st);
-    BTS_LAUNCH_CHECK();
-    return BTS_OK;
+    a.ldx = ldx; a.ldr = ldr; a.lds = lds; a.ldy = ldy; a.n = n; a.d = d; a.eps = eps; a.format = format; a.codes = codes; a.scales = scales;
+    // a wavefront a row up to 2048 elements (no barrier), a workgroup beyond
+    if (d <= 512) rms_norm_launch<T, 64, 1>(a, st);
+    else if (d <= 1024) rms_norm_launch<T, 64, 2>(a, st);
+    else if (d <= 2048) rms_norm_launch<T, 64, 4>(a, st);
+    else if (d <= 4096) rms_norm_launch<T, 256, 2>(a, st);
+    else if (d <= 8192) rms_norm_launch<T, 256, 4>(a, st);
+    else rms_norm_launch<T, 256, 0>(a, st);
 }
 
+template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> void tile_launch(const ProductArgs &p, hipStream_t st) {
+    const long tiles = (((long)p.n + TM - 1) / TM) * (((long)p.m + TN - 1) / TN);
+    hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK, AHEAD>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, st, p);
+}
+// Which kernel: by how many workgroups the sizes make of the chip, measured at d = 2048 unless said otherwise (us, E4M3 x E2M1).
+//  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 439 against
+//    630; 10000 x 2000, 320 tiles in two rounds: 61 against 55).  Two E4M3 operands' images of 256 rows do not fit.
+//  - 128 x 128 tiles from two a CU on (10000 x 2000: 56 against 75 with 64 x 64 ones; 2000 x 2000 x 1000, one a CU: 14.7 against 12.0).
+//  - 64 x 64 tiles from one a CU on (48 x 65536: 19; 1000 x 1000 x 1000: 6.6 against 11), below that 16 x 64 ones (200 x 2000 x 1024: 4.9 against
+//    6.0), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.5 against 18).
+//  - 16 x 16 tiles with the row split where there are fewer than two of them a CU (1 x 2000: 3.6 against 5.4).
 template <int FA, int FB> int product(bts_context *ctx, const ProductArgs &p, hipStream_t st) {
-    const long tiles = (((long)p.n + 31) / 32) * (((long)p.m + 31) / 32);
-    BTS_REQUIRE(tiles < (1L << 31), "n * m: too many tiles for one launch");
-    hipLaunchKernelGGL((k_mx_direct<FA, FB, 2, 2, 4>), dim3((unsigned)tiles), dim3(256), 0, st, p);
+    const auto tiles = [&](long a, long b) { return ((p.n + a - 1) / a) * ((p.m + b - 1) / b); };
+    const long cus = ctx->n_cu, t256 = tiles(256, 256), t128 = tiles(128, 128), most = 1L << 31;
+    BTS_REQUIRE(tiles(16, 16) < most, "n * m: too many tiles for one launch");
+    constexpr int SK = FA == E2M1 && FB == E2M1 ? 2 : 1;      // 128 bytes a row and stage
+    constexpr bool BIG = FA == E2M1 || FB == E2M1;
+    // 32-bit offsets inside a tile: 256 rows of codes, 128 rows of the output
+    const bool fits = (long)p.steps * 128 * 256 < most && p.ld * 4 * 128 < most && p.n < most - 256 && p.m < most - 256;
+    if (!fits || tiles(16, 16) < 2 * cus) hipLaunchKernelGGL((k_mx_direct<FA, FB>), dim3((unsigned)tiles(16, 16)), dim3(256), 0, st, p);
+    else if (p.n <= 32) tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
+    else if (p.m <= 32) tile_launch<FA, FB, 64, 16, 4, 1, 2, 2>(p, st);
+    else if (BIG && (t256 + cus - 1) / cus * cus * 4 * 2 <= t128 * 3) tile_launch<FA, FB, 256, BIG ? 256 : 128, FA == E2M1 ? 2 : 4, FA == E2M1 ? 4 : 2, 1, 1>(p, st);
+    else if (t128 >= 2 * cus) tile_launch<FA, FB, 128, 128, 2, 2, SK, 2>(p, st);
+    else if (tiles(64, 64) >= cus) tile_launch<FA, FB, 64, 64, 1, 4, SK, 2>(p, st);
+    else tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
     BTS_LAUNCH_CHECK();
     return BTS_OK;
 }
@@ -332,9 +594,12 @@ int bts_mx_quantize(bts_context *ctx, const void *x, int x_dtype, int ldx, int n
     BTS_REQUIRE(x && codes && scales, "null pointer");
     BTS_REQUIRE(aligned(x, dtype_bytes(x_dtype)) && aligned(codes, 16) && aligned(scales, 4), "x: element, codes: 16-byte, scales: 4-byte alignment");
     hipStream_t st = (hipStream_t)stream;
-    if (x_dtype == BTS_F32) return quantize(ctx, static_cast<const float *>(x), ldx, n, d, format, codes, scales, st);
-    if (x_dtype == BTS_F16) return quantize(ctx, static_cast<const _Float16 *>(x), ldx, n, d, format, codes, scales, st);
-    return quantize(ctx, static_cast<const bf16 *>(x), ldx, n, d, format, codes, scales, st);
+    BTS_REQUIRE(pieces(n, d) <= MOST_PIECES, "n * d: too many elements for one call");
+    if (x_dtype == BTS_F32) quantize<float>(ctx, x, ldx, n, d, format, codes, scales, st);
+    else if (x_dtype == BTS_F16) quantize<_Float16>(ctx, x, ldx, n, d, format, codes, scales, st);
+    else quantize<bf16>(ctx, x, ldx, n, d, format, codes, scales, st);
+    BTS_LAUNCH_CHECK();
+    return BTS_OK;
 }
 
 int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *scales, int format, int n, int d, void *out, int out_dtype,
@@ -346,9 +611,12 @@ int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *sca
     BTS_REQUIRE(out && codes && scales, "null pointer");
     BTS_REQUIRE(aligned(out, dtype_bytes(out_dtype)) && aligned(codes, 16) && aligned(scales, 4), "out: element, codes: 16-byte, scales: 4-byte alignment");
     hipStream_t st = (hipStream_t)stream;
-    if (out_dtype == BTS_F32) return dequantize(ctx, codes, scales, format, n, d, static_cast<float *>(out), ldo, st);
-    if (out_dtype == BTS_F16) return dequantize(ctx, codes, scales, format, n, d, static_cast<_Float16 *>(out), ldo, st);
-    return dequantize(ctx, codes, scales, format, n, d, static_cast<bf16 *>(out), ldo, st);
+    BTS_REQUIRE(pieces(n, d) <= MOST_PIECES, "n * d: too many elements for one call");
+    if (out_dtype == BTS_F32) dequantize<float>(ctx, codes, scales, format, n, d, out, ldo, st);
+    else if (out_dtype == BTS_F16) dequantize<_Float16>(ctx, codes, scales, format, n, d, out, ldo, st);
+    else dequantize<bf16>(ctx, codes, scales, format, n, d, out, ldo, st);
+    BTS_LAUNCH_CHECK();
+    return BTS_OK;
 }
 
 int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d,
@@ -374,9 +642,11 @@ int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void
     BTS_REQUIRE(aligned(codes, 16) && aligned(scales, 4), "codes: 16-byte, scales: 4-byte alignment");
     hipStream_t st = (hipStream_t)stream;
     const int f = codes ? format : -1;
-    if (dtype == BTS_F32) return rms_norm<float>(x, ldx, residual, ldr, weight, n, d, (float)eps, sum, lds, y, ldy, f, codes, scales, st);
-    if (dtype == BTS_F16) return rms_norm<_Float16>(x, ldx, residual, ldr, weight, n, d, (float)eps, sum, lds, y, ldy, f, codes, scales, st);
-    return rms_norm<bf16>(x, ldx, residual, ldr, weight, n, d, (float)eps, sum, lds, y, ldy, f, codes, scales, st);
+    if (dtype == BTS_F32) rms_norm<float>(x, ldx, residual, ldr, weight, n, d, eps, sum, lds, y, ldy, f, codes, scales, st);
+    else if (dtype == BTS_F16) rms_norm<_Float16>(x, ldx, residual, ldr, weight, n, d, eps, sum, lds, y, ldy, f, codes, scales, st);
+    else rms_norm<bf16>(x, ldx, residual, ldr, weight, n, d, eps, sum, lds, y, ldy, f, codes, scales, st);
+    BTS_LAUNCH_CHECK();
+    return BTS_OK;
 }
 
 int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_scales, int a_format, int n, const uint8_t *b_codes,
@@ -397,7 +667,7 @@ int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_sc
     p.n = n; p.m = m; p.steps = (int)(padded(d) / MX_ROW);
     p.alpha = (float)alpha; p.floor_zero = floor_zero != 0;
     p.out = out; p.out_dtype = out_dtype; p.ld = ld;
-    p.out_vec = aligned(out, 4 * b) && ld % 4 == 0;
+    p.out_vec = aligned(out, 16) && (size_t)ld * b % 16 == 0;
     hipStream_t st = (hipStream_t)stream;
     if (a_format == E2M1) return b_format == E2M1 ? product<E2M1, E2M1>(ctx, p, st) : product<E2M1, E4M3>(ctx, p, st);
     return b_format == E2M1 ? product<E4M3, E2M1>(ctx, p, st) : product<E4M3, E4M3>(ctx, p, st);

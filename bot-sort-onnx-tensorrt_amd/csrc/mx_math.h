@@ -38,36 +38,78 @@ template <> __device__ __forceinline__ bf16 from_f32<bf16>(float v) {      // ne
 }
 
 // ---- 8 consecutive elements of a row ------------------------------------------------------------------------------------------
-// VEC: the address is 16-byte aligned and all 8 exist (the caller's rule); otherwise element by element, zeros behind the end.
-template <class T, bool VEC> __device__ __forceinline__ void load8(const T *p, int have, float (&v)[8]) {
-    if (VEC) {
-        struct alignas(16) Pack { T e[16 / sizeof(T)]; };
+// All 8 there: 16 bytes an access whatever the address is a multiple of (the part reads and writes unaligned; rows of odd width
+// element by element took twice the time); otherwise element by element, zeros behind the end.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+// two values as one word of a 16-bit type (one conversion instruction for two bfloat16)
+template <class T> __device__ __forceinline__ uint32_t pack2(float a, float b) {
+#if !defined(BTS_HOST_EMU)
+    if constexpr (__is_same(T, bf16)) {
+        typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2{a, b}, bf16x2));
+    }
+#endif
+    return __builtin_bit_cast(uint16_t, from_f32<T>(a)) | (uint32_t)__builtin_bit_cast(uint16_t, from_f32<T>(b)) << 16;
+}
+// v rounded to T and back
+template <class T> __device__ __forceinline__ void round8(float (&v)[8]) {
+    if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k) {
-            const Pack q = reinterpret_cast<const Pack *>(p)[k];
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t w = pack2<T>(v[2 * k], v[2 * k + 1]);
+            v[2 * k] = to_f32(__builtin_bit_cast(T, (uint16_t)w));
+            v[2 * k + 1] = to_f32(__builtin_bit_cast(T, (uint16_t)(w >> 16)));
+        }
+    }
+}
+template <class T> __device__ __forceinline__ void load8(const T *p, int have, float (&v)[8]) {
+    if (have >= 8) {
+        const u32x4 a = *reinterpret_cast<const u32x4_any *>(p);
+        if constexpr (sizeof(T) == 4) {
+            const u32x4 b = *reinterpret_cast<const u32x4_any *>(p + 4);
 #pragma unroll
-            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) v[k * (int)(16 / sizeof(T)) + e] = to_f32(q.e[e]);
+            for (int k = 0; k < 4; ++k) { v[k] = bits_f32(a[k]); v[4 + k] = bits_f32(b[k]); }
+        } else {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                v[2 * k] = to_f32(__builtin_bit_cast(T, (uint16_t)a[k]));
+                v[2 * k + 1] = to_f32(__builtin_bit_cast(T, (uint16_t)(a[k] >> 16)));
+            }
         }
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = e < have ? to_f32(p[e]) : 0.0f;
+        for (int k = 0; k < 8; ++k) v[k] = k < have ? to_f32(p[k]) : 0.0f;
     }
 }
-template <class T, bool VEC> __device__ __forceinline__ void store8(T *p, int have, const float (&v)[8]) {
-    if (VEC) {
-        struct alignas(16) Pack { T e[16 / sizeof(T)]; };
+// 8 elements as the words they are stored in (float: 8 words, 16-bit types: 4)
+template <class T> struct Words { uint32_t w[2 * sizeof(T)]; };
+template <class T> __device__ __forceinline__ Words<T> to_words(const float (&v)[8]) {
+    Words<T> r;
+    if constexpr (sizeof(T) == 4) {
 #pragma unroll
-        for (int k = 0; k < (int)(8 * sizeof(T) / 16); ++k) {
-            Pack q;
-#pragma unroll
-            for (int e = 0; e < (int)(16 / sizeof(T)); ++e) q.e[e] = from_f32<T>(v[k * (int)(16 / sizeof(T)) + e]);
-            reinterpret_cast<Pack *>(p)[k] = q;
-        }
+        for (int k = 0; k < 8; ++k) r.w[k] = f32_bits(v[k]);
     } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) if (e < have) p[e] = from_f32<T>(v[e]);
+        for (int k = 0; k < 4; ++k) r.w[k] = pack2<T>(v[2 * k], v[2 * k + 1]);
+    }
+    return r;
+}
+template <class T> __device__ __forceinline__ void store_words(T *p, int have, const Words<T> &x) {
+    if (have >= 8) {
+        *reinterpret_cast<u32x4_any *>(p) = u32x4{x.w[0], x.w[1], x.w[2], x.w[3]};
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<u32x4_any *>(p + 4) = u32x4{x.w[4], x.w[5], x.w[6], x.w[7]};
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            if (k >= have) continue;
+            if constexpr (sizeof(T) == 4) p[k] = bits_f32(x.w[k]);
+            else p[k] = __builtin_bit_cast(T, (uint16_t)(x.w[k / 2] >> (16 * (k & 1))));
+        }
     }
 }
+template <class T> __device__ __forceinline__ void store8(T *p, int have, const float (&v)[8]) { store_words<T>(p, have, to_words<T>(v)); }
 
 // ---- quantisation -------------------------------------------------------------------------------------------------------------
 // The scale byte of a block from the bits of its largest magnitude: floor(log2) is the exponent field (a subnormal's field, 0, and
@@ -93,7 +135,7 @@ template <int FMT> __device__ __forceinline__ uint2 encode8(const float (&v)[8])
     } else {
         float w[8];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) w[e] = fminf(fmaxf(v[e], -448.0f), 448.0f);
+        for (int e = 0; e < 8; ++e) w[e] = __builtin_amdgcn_fmed3f(v[e], -448.0f, 448.0f);
         int a = 0, b = 0;
         a = __builtin_amdgcn_cvt_pk_fp8_f32(w[0], w[1], a, false);
         a = __builtin_amdgcn_cvt_pk_fp8_f32(w[2], w[3], a, true);
@@ -109,24 +151,37 @@ template <int FMT> __device__ __forceinline__ uint2 encode_block(const float (&v
     uint32_t top = 0;                    // magnitudes compare like their bits; a NaN's are above an infinity's
 #pragma unroll
     for (int e = 0; e < 8; ++e) top = max(top, f32_bits(v[e]) & 0x7fffffffu);
-    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
-    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xf, 0xf, false));      // lane ^ 1
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xf, 0xf, false));      // lane ^ 2
     sbyte = scale_byte<FMT>(top);
     const float inv = scale_inverse(sbyte == 255 ? 254 : sbyte);
     float w[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) w[e] = sbyte == 255 ? 0.0f : v[e] * inv;
-    return encode8<FMT>(w);
+    for (int e = 0; e < 8; ++e) w[e] = v[e] * inv;
+    const uint2 c = encode8<FMT>(w);
+    return uint2{sbyte == 255 ? 0u : c.x, sbyte == 255 ? 0u : c.y};
 }
 
 // ---- decoding -----------------------------------------------------------------------------------------------------------------
-// The code's exponent and fraction bits, put where a float32 has its own, are the value times 2^-126 (E2M1) or 2^-120 (E4M3),
-// subnormal codes included; two exact products give the value.
-template <int FMT> __device__ __forceinline__ float decode1(uint32_t c) {
-    if (FMT == E2M1) return bits_f32(((c & 7u) << 22) | ((c & 8u) << 28)) * bits_f32((126u + 127u) << 23);
-    const float v = bits_f32(((c & 127u) << 20) | ((c & 128u) << 24)) * bits_f32((120u + 127u) << 23);
-    return (c & 127u) == 127u ? bits_f32(0x7fc00000u) : v;
+// 8 packed codes of one block -> the words they are stored as.  The conversion instructions multiply by the scale, whose byte they take
+// from a float32's exponent field (byte 0 is 2^-127 to them and 255 a NaN, as in the format), and round once to the output's type.
+template <class T, int FMT> __device__ __forceinline__ Words<T> decode8(uint2 c, int sbyte) {
+    const float s = bits_f32((uint32_t)sbyte << 23);
+    Words<T> r;
+#define MX_PAIR(k, word, sel4, sel8)                                                                                                              \
+    if constexpr (sizeof(T) == 4) {                                                                                                               \
+        const f32x2 p = FMT == E2M1 ? __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c.x, s, sel4) : __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(word, s, sel8); \
+        r.w[2 * k] = f32_bits(p[0]); r.w[2 * k + 1] = f32_bits(p[1]);                                                                              \
+    } else if constexpr (__is_same(T, _Float16))                                                                                                   \
+        r.w[k] = __builtin_bit_cast(uint32_t, FMT == E2M1 ? __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c.x, s, sel4) : __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(word, s, sel8)); \
+    else                                                                                                                                          \
+        r.w[k] = __builtin_bit_cast(uint32_t, FMT == E2M1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c.x, s, sel4) : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(word, s, sel8));
+    MX_PAIR(0, c.x, 0, false)
+    MX_PAIR(1, c.x, 1, true)
+    MX_PAIR(2, c.y, 2, false)
+    MX_PAIR(3, c.y, 3, true)
+#undef MX_PAIR
+    return r;
 }
-__device__ __forceinline__ float scale_value(int s) { return s == 255 ? bits_f32(0x7fc00000u) : bits_f32(s == 0 ? 0x00400000u : (uint32_t)s << 23); }
 
 }  // namespace mx

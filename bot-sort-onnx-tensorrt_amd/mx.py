@@ -10,13 +10,26 @@ import ctypes
 
 from . import _lib
 
+torch = None                            # imported by the first call: importing the package does not
+_DTYPES = {}                            # enum bts_dtype
+_raw_stream = None
 _FORMATS = {"e2m1": 0, "e4m3": 1}       # enum bts_mx_format
 _ROW, _BLOCK = 128, 32                  # elements a row is padded to; elements per scale
 
 
+def _init():
+    global torch, _raw_stream
+    import torch as t
+    _DTYPES.update({t.float32: 1, t.float16: 2, t.bfloat16: 3})
+    # the number of a device's current stream without the Stream object around it (2 us of a 10 us call)
+    _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None)
+    torch = t
+
+
 def _dtype_code(dtype):
-    import torch
-    code = {torch.float32: 1, torch.float16: 2, torch.bfloat16: 3}.get(dtype)      # enum bts_dtype
+    if torch is None:
+        _init()
+    code = _DTYPES.get(dtype)
     if code is None:
         raise _lib.BtsError("mx rows: float32, float16 or bfloat16 expected, got %s" % (dtype,))
     return code
@@ -36,9 +49,11 @@ def _rows2d(t, name, like=None):
     if t.dim() != 2:
         raise _lib.BtsError("%s: [rows, d] expected, got %d dimensions" % (name, t.dim()))
     n, d = t.shape
-    ld = t.stride(0) if n > 1 else max(d, 1)
-    if (t.stride(1) != 1 and d > 1) or ld < d:
-        raise _lib.BtsError("%s: the elements of a row must be adjacent and rows may not overlap (strides %s): call .contiguous()" % (name, tuple(t.stride())))
+    ld, unit = t.stride()
+    if n <= 1:
+        ld = max(d, 1)
+    if (unit != 1 and d > 1) or ld < d:
+        raise _lib.BtsError("%s: the elements of a row must be adjacent and rows may not overlap (strides %s): call .contiguous()" % (name, t.stride()))
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
         raise _lib.BtsError("%s: shape, type and device of x expected (%s %s %s)" % (name, tuple(like.shape), like.dtype, like.device))
     return t.data_ptr(), ld
@@ -46,9 +61,10 @@ def _rows2d(t, name, like=None):
 
 def _call(device):
     """(library, context handle, stream) of a device's current stream."""
-    import torch
-    lib = _lib.load()
-    return lib, _lib.default_context(device.index).handle, torch.cuda.current_stream(device).cuda_stream
+    index = device.index
+    ctx = _lib._default_ctx.get(index) or _lib.default_context(index)
+    stream = torch.cuda.current_stream(device).cuda_stream if index is None or _raw_stream is None else _raw_stream(index)
+    return _lib.load(), ctx.handle, stream
 
 
 def mx_row_bytes(fmt: str, d: int) -> "tuple[int, int]":
@@ -65,7 +81,8 @@ class MxRows:
     __slots__ = ("codes", "scales", "d", "fmt", "_code")
 
     def __init__(self, codes, scales, d: int, fmt: str):
-        import torch
+        if torch is None:
+            _init()
         self._code = _format_code(fmt)
         d = int(d)
         if d <= 0:
@@ -82,6 +99,13 @@ class MxRows:
             raise _lib.BtsError("MxRows: contiguous codes and scales expected")
         self.codes, self.scales, self.d, self.fmt = codes, scales, d, fmt
 
+    @classmethod
+    def _of(cls, codes, scales, d, fmt, code):
+        """Rows of tensors that this module has made itself."""
+        self = cls.__new__(cls)
+        self.codes, self.scales, self.d, self.fmt, self._code = codes, scales, d, fmt, code
+        return self
+
     def __len__(self):
         return self.codes.shape[0]
 
@@ -91,14 +115,19 @@ class MxRows:
     @classmethod
     def empty(cls, n: int, d: int, fmt: str, device="cuda") -> "MxRows":
         """Room for n rows."""
-        import torch
-        c, s = mx_row_bytes(fmt, d)
+        if torch is None:
+            _init()
+        code, wide = _format_code(fmt), (int(d) + _ROW - 1) // _ROW * _ROW
+        if wide <= 0:
+            raise _lib.BtsError("MxRows: d must be positive")
         device = torch.device(device)
-        return cls(torch.empty((int(n), c), dtype=torch.uint8, device=device), torch.empty((int(n), s), dtype=torch.uint8, device=device), d, fmt)
+        return cls._of(torch.empty((n, wide // 2 if code == 0 else wide), dtype=torch.uint8, device=device),
+                       torch.empty((n, wide // _BLOCK), dtype=torch.uint8, device=device), int(d), fmt, code)
 
     def dequantize(self, dtype=None):
         """[n, d] of the values held (float32 unless `dtype` says otherwise)."""
-        import torch
+        if torch is None:
+            _init()
         dtype = torch.float32 if dtype is None else dtype
         code = _dtype_code(dtype)
         n, d = self.codes.shape[0], self.d
@@ -132,7 +161,6 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     -> (rows in `fmt`, h).  fmt=None: no quantised rows, only `y_out`.
 
     `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` the normalised rows in x's type."""
-    import torch
     px, ldx = _rows2d(x, "x")
     dt = _dtype_code(x.dtype)
     n, d = x.shape
@@ -158,7 +186,6 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
 
     `dtype`: float32 (the default) where both are e2m1; float16 / bfloat16 for any (the default with an e4m3 operand is bfloat16).
     `out`: a matrix to fill (its type counts; rows may be strided)."""
-    import torch
     if not isinstance(a, MxRows) or not isinstance(b, MxRows):
         raise _lib.BtsError("mx_product: MxRows expected")
     device = a.codes.device

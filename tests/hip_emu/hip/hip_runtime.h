@@ -92,6 +92,9 @@ static inline void __syncthreads() { emu::barrier(); }
 static inline int __syncthreads_or(int v) { return emu::barrier_or(v); }
 static inline void __threadfence() {}
 #define __builtin_amdgcn_fence(...) ((void)0)
+#define __builtin_amdgcn_sched_barrier(n) ((void)0)
+#define __builtin_amdgcn_sched_group_barrier(mask, n, id) ((void)0)
+#define __builtin_amdgcn_s_setprio(n) ((void)0)
 #define __builtin_amdgcn_s_sleep(n) emu::spin()      /* only used inside spin-waits on another workgroup */
 #define __builtin_amdgcn_wave_barrier() ((void)emu::collective(emu::OP_WAVE_BARRIER, __COUNTER__, 0, 0, 0, 0))
 static inline unsigned long long __builtin_amdgcn_s_memrealtime() { static unsigned long long t = 0; return t += 1; }
@@ -250,6 +253,66 @@ static inline int emu_cvt_pk_fp8(float a, float b, int old, bool high) {
 }
 #define __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, scale, sel) emu_cvt_pk_fp4((old), (a), (b), (scale), (sel))
 #define __builtin_amdgcn_cvt_pk_fp8_f32(a, b, old, high) emu_cvt_pk_fp8((a), (b), (old), (high))
+// raw buffers: a base, a size in bytes; what does not lie inside reads as zeros
+struct __amdgpu_buffer_rsrc_t { const char *base; unsigned size; };
+typedef unsigned emu_u32x4 __attribute__((ext_vector_type(4)));
+static inline __amdgpu_buffer_rsrc_t emu_make_rsrc(const void *p, int size) { return {(const char *)p, (unsigned)size}; }
+template <class T> static inline T emu_buffer_load(__amdgpu_buffer_rsrc_t r, int at) {
+    T v;
+    memset(&v, 0, sizeof(T));
+    if ((uint64_t)(unsigned)at + sizeof(T) <= r.size) memcpy(&v, r.base + (unsigned)at, sizeof(T));
+    return v;
+}
+#define __builtin_amdgcn_raw_buffer_load_b128(r, at, base, aux) emu_buffer_load<emu_u32x4>((r), (at) + (base))
+#define __builtin_amdgcn_raw_buffer_load_b32(r, at, base, aux) emu_buffer_load<unsigned>((r), (at) + (base))
+#define __builtin_amdgcn_make_buffer_rsrc(p, stride, size, flags) emu_make_rsrc((p), (size))
+// ... and the same from a buffer to LDS: lane l's bytes land at base + size l, asynchronously like global_load_lds below
+static inline void emu_buffer_load_lds(__amdgpu_buffer_rsrc_t r, void *lds_base, int size, int at);
+#define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, size, at, base, off, aux) emu_buffer_load_lds((r), (void *)(lds), (size), (at) + (base) + (off))
+static inline unsigned emu_perm(unsigned hi, unsigned lo, unsigned sel) {
+    unsigned out = 0;
+    for (int k = 0; k < 4; ++k) {
+        const unsigned s = (sel >> (8 * k)) & 255;
+        if (s < 8) out |= (((s < 4 ? lo : hi) >> (8 * (s & 3))) & 255u) << (8 * k);      /* 12: a zero byte */
+    }
+    return out;
+}
+#define __builtin_amdgcn_perm(hi, lo, sel) emu_perm((hi), (lo), (sel))
+// conversions of two codes back: value * 2^(exponent field of the scale - 127), rounded once to the output's type
+typedef float emu_f32x2 __attribute__((ext_vector_type(2)));
+static inline double emu_scaled(int fmt, unsigned code, float scale) {
+    unsigned b;
+    memcpy(&b, &scale, 4);
+    const int s = (b >> 23) & 255;
+    return s == 255 ? (double)NAN : emu_f8f6f4(fmt, (int)code) * ldexp(1.0, s - 127);
+}
+static inline unsigned emu_code(int fmt, unsigned src, int sel, int k) { return fmt == 4 ? (src >> (8 * sel + 4 * k)) & 15u : (src >> (16 * sel + 8 * k)) & 255u; }
+static inline emu_f32x2 emu_cvt_f32(int fmt, unsigned src, float scale, int sel) {
+    return emu_f32x2{(float)emu_scaled(fmt, emu_code(fmt, src, sel, 0), scale), (float)emu_scaled(fmt, emu_code(fmt, src, sel, 1), scale)};
+}
+static inline unsigned emu_cvt_f16(int fmt, unsigned src, float scale, int sel) {
+    unsigned r = 0;
+    for (int k = 0; k < 2; ++k) { const _Float16 h = (_Float16)(float)emu_scaled(fmt, emu_code(fmt, src, sel, k), scale); uint16_t b; memcpy(&b, &h, 2); r |= (unsigned)b << (16 * k); }
+    return r;
+}
+static inline unsigned emu_cvt_bf16(int fmt, unsigned src, float scale, int sel) {
+    unsigned r = 0;
+    for (int k = 0; k < 2; ++k) {
+        const float f = (float)emu_scaled(fmt, emu_code(fmt, src, sel, k), scale);
+        unsigned b;
+        memcpy(&b, &f, 4);
+        b = f != f ? 0x7fc0u : (b + 0x7fffu + ((b >> 16) & 1u)) >> 16;
+        r |= b << (16 * k);
+    }
+    return r;
+}
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(c, s, sel) emu_cvt_f32(4, (c), (s), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_f32_fp8(c, s, sel) emu_cvt_f32(0, (c), (s), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp4(c, s, sel) emu_cvt_f16(4, (c), (s), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, s, sel) emu_cvt_f16(0, (c), (s), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(c, s, sel) emu_cvt_bf16(4, (c), (s), (sel))
+#define __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, s, sel) emu_cvt_bf16(0, (c), (s), (sel))
+#define __builtin_amdgcn_fmed3f(v, lo, hi) fminf(fmaxf((v), (lo)), (hi))
 // (only named inside a discarded `if constexpr` branch of a timing experiment)
 #define __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(a, b, c, ...) (c)
 // global_load_lds (16 B per lane): the LDS image is lane-linear from the wave-uniform base -- lane l's bytes land at base + 16 l.
@@ -268,6 +331,11 @@ void lds_dma_check(const void *p, int n, const char *what);    // an LDS read / 
 }
 static inline void emu_global_load_lds(const void *g, void *lds_base, int size) {
     emu::lds_dma_issue(g, (char *)lds_base + (size_t)(emu::tid_x() & 63) * (size_t)size, size);
+}
+static inline void emu_buffer_load_lds(__amdgpu_buffer_rsrc_t r, void *lds_base, int size, int at) {
+    static const char zeros[16] = {0};
+    const bool inside = (uint64_t)(unsigned)at + (unsigned)size <= r.size;
+    emu::lds_dma_issue(inside ? (const void *)(r.base + (unsigned)at) : (const void *)zeros, (char *)lds_base + (size_t)(emu::tid_x() & 63) * (size_t)size, size);
 }
 #define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) emu_global_load_lds((const void *)(g), (void *)(l), (size))
 

@@ -306,7 +306,8 @@ def feature_rows(n, d, seed):
 
 FMTS = list(itertools.product(["e2m1", "e4m3"], ["e2m1", "e4m3"]))
 PRODUCTS = [(1, 1, 1), (1, 300, 64), (16, 17, 128), (17, 1, 300), (33, 65, 500), (5, 130, 1111), (64, 64, 256), (100, 37, 129)]
-BIG = [(1, 5000, 2048), (3, 70001, 96), (40, 2000, 1024), (200, 333, 4100), (512, 256, 256), (777, 1300, 640), (1500, 1025, 2048), (2500, 4, 512), (33000, 40, 200)]
+BIG = [(1, 5000, 2048), (3, 70001, 96), (40, 2000, 1024), (200, 333, 4100), (512, 256, 256), (777, 1300, 640), (1500, 1025, 2048), (2500, 4, 512), (33000, 40, 200),
+       (9000, 20, 700), (2000, 1999, 300), (3000, 2900, 300), (4000, 4090, 300), (4096, 4096, 129)]
 
 
 def run_product(bts, n, m, d, fa, fb, out):
