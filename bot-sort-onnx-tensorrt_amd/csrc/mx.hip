@@ -57,11 +57,13 @@ template <class T> struct NormArgs {
     uint8_t *codes, *scales;
 };
 
-template <class T> __device__ __forceinline__ void norm_load(const NormArgs<T> &a, long i, int k, float (&h)[8]) {
-    load8(a.x + i * a.ldx + k, a.d - k, h);
+// WHOLE: d is a multiple of 8, so every piece is (the tails' code, five times a piece, is most of the kernel otherwise)
+template <class T, bool WHOLE> __device__ __forceinline__ void norm_load(const NormArgs<T> &a, long i, int k, float (&h)[8]) {
+    const int have = WHOLE ? 8 : a.d - k;
+    load8(a.x + i * a.ldx + k, have, h);
     if (!a.residual) return;
     float r[8];
-    load8(a.residual + i * a.ldr + k, a.d - k, r);
+    load8(a.residual + i * a.ldr + k, have, r);
     // the sum is rounded to its stored type first and normalised from there: whoever reads it back gets the same row
 #pragma unroll
     for (int e = 0; e < 8; ++e) h[e] += r[e];
@@ -73,17 +75,18 @@ __device__ __forceinline__ double squares(const float (&h)[8]) {
     return (double)(((h[0] * h[0] + h[1] * h[1]) + (h[2] * h[2] + h[3] * h[3])) + ((h[4] * h[4] + h[5] * h[5]) + (h[6] * h[6] + h[7] * h[7])));
 }
 // the normalised piece at column k: to y, and as codes (whole blocks: a block's four lanes come together)
-template <class T> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, float inv, float (&h)[8]) {
+template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, float inv, float (&h)[8]) {
     if (k < a.d) {
+        const int have = WHOLE ? 8 : a.d - k;
         if (a.weight) {
             float w[8];
-            load8(a.weight + k, a.d - k, w);
+            load8(a.weight + k, have, w);
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[e] *= w[e];             // (exact for 16-bit types: one rounding, that of the factor, follows)
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = k + e < a.d ? h[e] * inv : 0.0f;
-        if (a.y) store8(a.y + i * a.ldy + k, a.d - k, h);
+        for (int e = 0; e < 8; ++e) h[e] = WHOLE || e < have ? h[e] * inv : 0.0f;
+        if (a.y) store8(a.y + i * a.ldy + k, have, h);
     }
     if (a.format < 0) return;
     int s;
@@ -95,8 +98,8 @@ template <class T> __device__ __forceinline__ void norm_emit(const NormArgs<T> &
 
 // TPR threads per row, CH pieces of 8 elements a thread: the row stays in registers between the sum and the output, so x and residual
 // are read once.  CH = 0: rows beyond 8192 elements, in two passes; the second reads the stored sum, or x and residual again.
-// One pass over memory bounds it (32768 x 4096 bfloat16 with residual and weight: 0.94 GB).
-template <class T, int TPR, int CH>
+// One pass over memory bounds it: 32768 x 4096 bfloat16 with residual and weight, 0.94 GB in 163 us (5.8 TB/s).
+template <class T, int TPR, int CH, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
     __shared__ double part[4];
     const long i = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
@@ -110,18 +113,18 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
             const int k = first + c * TPR * 8;
 #pragma unroll
             for (int e = 0; e < 8; ++e) h[c][e] = 0.0f;
-            if (k < a.d) norm_load(a, i, k, h[c]);
+            if (k < a.d) norm_load<T, WHOLE>(a, i, k, h[c]);
         }
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = first + c * TPR * 8;
-            if (a.sum && k < a.d) store8(a.sum + i * a.lds + k, a.d - k, h[c]);
+            if (a.sum && k < a.d) store8(a.sum + i * a.lds + k, WHOLE ? 8 : a.d - k, h[c]);
             ss += squares(h[c]);
         }
     } else {
         for (int k = first; k < a.d; k += TPR * 8) {
-            norm_load(a, i, k, h[0]);
-            if (a.sum) store8(a.sum + i * a.lds + k, a.d - k, h[0]);
+            norm_load<T, WHOLE>(a, i, k, h[0]);
+            if (a.sum) store8(a.sum + i * a.lds + k, WHOLE ? 8 : a.d - k, h[0]);
             ss += squares(h[0]);
         }
     }
@@ -137,16 +140,16 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = first + c * TPR * 8;
-            if (k < width) norm_emit(a, i, k, width, inv, h[c]);
+            if (k < width) norm_emit<T, WHOLE>(a, i, k, width, inv, h[c]);
         }
     } else {
         for (int k = first; k < width; k += TPR * 8) {
             if (k >= a.d) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) h[0][e] = 0.0f;
-            } else if (a.sum) load8(a.sum + i * a.lds + k, a.d - k, h[0]);
-            else norm_load(a, i, k, h[0]);
-            norm_emit(a, i, k, width, inv, h[0]);
+            } else if (a.sum) load8(a.sum + i * a.lds + k, WHOLE ? 8 : a.d - k, h[0]);
+            else norm_load<T, WHOLE>(a, i, k, h[0]);
+            norm_emit<T, WHOLE>(a, i, k, width, inv, h[0]);
         }
     }
 }
@@ -204,34 +207,23 @@ template <int FA, int FB> __device__ __forceinline__ v4f mma_bytes(v8i fb, v8i f
     }
 }
 
-template <class T> __device__ __forceinline__ void store_out4(T *p, int have, bool vec, const float (&v)[4]) {
-    if (vec && have >= 4) {
-        struct alignas(sizeof(T) * 4) Pack { T e[4]; } q;
+// the factor and the floor of N results (a NaN stays one)
+template <int N> __device__ __forceinline__ void finish(const ProductArgs &p, float (&v)[N]) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) q.e[e] = from_f32<T>(v[e]);
-        *reinterpret_cast<Pack *>(p) = q;
-    } else {
+    for (int e = 0; e < N; ++e) v[e] *= p.alpha;
+    if (p.floor_zero) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) if (e < have) p[e] = from_f32<T>(v[e]);
+        for (int e = 0; e < N; ++e) v[e] = v[e] < 0.0f ? 0.0f : v[e];
     }
 }
-__device__ __forceinline__ void finish(const ProductArgs &p, v4f acc, float (&v)[4]) {
+// four consecutive columns j .. j + 3 of row i, element by element
+template <class T> __device__ __forceinline__ void epilogue4(const ProductArgs &p, long i, long j, v4f acc) {
+    if (i >= p.n) return;
+    float v[4] = {acc[0], acc[1], acc[2], acc[3]};
+    finish(p, v);
+    T *const to = static_cast<T *>(p.out) + i * p.ld + j;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-        v[e] = acc[e] * p.alpha;
-        if (p.floor_zero) v[e] = v[e] < 0.0f ? 0.0f : v[e];       // (a NaN stays one)
-    }
-}
-// four consecutive columns j .. j + 3 of row i
-__device__ __forceinline__ void epilogue4(const ProductArgs &p, long i, int j, v4f acc) {
-    if (i >= p.n || j >= p.m) return;
-    float v[4];
-    finish(p, acc, v);
-    const long at = i * p.ld + j;
-    const int have = p.m - j;
-    if (p.out_dtype == BTS_F32) store_out4(static_cast<float *>(p.out) + at, have, p.out_vec, v);
-    else if (p.out_dtype == BTS_F16) store_out4(static_cast<_Float16 *>(p.out) + at, have, p.out_vec, v);
-    else store_out4(static_cast<bf16 *>(p.out) + at, have, p.out_vec, v);
+    for (int e = 0; e < 4; ++e) if (j + e < p.m) to[e] = from_f32<T>(v[e]);
 }
 
 // A workgroup of 4 wavefronts computes one 16 x 16 tile straight from memory; each wavefront takes a quarter of the row, and the parts are
@@ -254,7 +246,9 @@ __global__ __launch_bounds__(256) void k_mx_direct(ProductArgs p) {
     __syncthreads();
     if (wave > 0) return;
     acc = ((acc + part[0][lane]) + part[1][lane]) + part[2][lane];
-    epilogue4(p, ti * 16 + r, (int)tj * 16 + 4 * g, acc);
+    if (p.out_dtype == BTS_F32) epilogue4<float>(p, ti * 16 + r, tj * 16 + 4 * g, acc);
+    else if (p.out_dtype == BTS_F16) epilogue4<_Float16>(p, ti * 16 + r, tj * 16 + 4 * g, acc);
+    else epilogue4<bf16>(p, ti * 16 + r, tj * 16 + 4 * g, acc);
 }
 
 // XCD-aware order of the tiles: the 8 XCDs have an L2 each and take workgroups in turn, so every XCD gets a contiguous run of tiles, and a
@@ -274,6 +268,7 @@ struct TileRows {
         rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t *>(base + (long)row * stride), 0, min(tile, rows - row) * stride, 0x00020000);
     }
     __device__ __forceinline__ v4i load16(int at) const { return __builtin_bit_cast(v4i, __builtin_amdgcn_raw_buffer_load_b128(rsrc, at, 0, 0)); }
+    static constexpr int BEHIND = 0x7ffffff0;
     __device__ __forceinline__ uint32_t load4(int at) const { return __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0); }
 };
 
@@ -338,12 +333,16 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
     for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int w0 = 0; w0 < CT; w0 += FRAGS) {
+            float v[FRAGS * 4];
+#pragma unroll
+            for (int e = 0; e < FRAGS * 4; ++e) v[e] = acc[u][w0 + e / 4][e % 4];
+            finish(p, v);
 #pragma unroll
             for (int w = 0; w < FRAGS; ++w) {
-                float v[4];
-                finish(p, acc[u][w0 + w], v);
                 const int at = (w * 16 + 4 * g) * (int)sizeof(T);
-                store_out4(reinterpret_cast<T *>(room + r * ROWB + ((at / 16) ^ (r & (CHUNKS - 1))) * 16 + at % 16), 4, true, v);
+                uint8_t *const to = room + r * ROWB + ((at / 16) ^ (r & (CHUNKS - 1))) * 16 + at % 16;
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<v4f *>(to) = v4f{v[4 * w], v[4 * w + 1], v[4 * w + 2], v[4 * w + 3]};
+                else *reinterpret_cast<uint2 *>(to) = uint2{pack2<T>(v[4 * w], v[4 * w + 1]), pack2<T>(v[4 * w + 2], v[4 * w + 3])};
             }
             __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
             __builtin_amdgcn_wave_barrier();
@@ -387,7 +386,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     __shared__ __attribute__((aligned(1024))) uint8_t image[IMAGES > ROOM ? IMAGES : ROOM];
     // scale bytes: [group][lane group][row of a fragment][fragment], so that a lane's four are one word
     __shared__ __attribute__((aligned(16))) uint8_t lscale[2][SK][GA + GB][4][16][4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
     const int first_a = 8 * (wm * RT % 4), first_b = 8 * (wn * CT % 4);      // where a wavefront's fragments begin in their group's words
     int tm, tn;
@@ -400,17 +399,21 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     OpB b;
     a.init(tid, wm * RT * 16, r, g, stride_a);
     b.init(tid, wn * CT * 16, r, g, stride_b);
-    // (depths behind the row's end load the next row's beginning, or zeros; they are not multiplied)
+    // (Depths behind the row's end load the next row's beginning, or zeros; they are not multiplied.  Nor is the one stage behind it that the
+    // phased form loads rather than branch between its reads.)
     struct Stage { typename OpA::Regs a; typename OpB::Regs b; uint32_t scale[SMOVES]; };
     const auto load = [&](Stage &st, int stage) {
-        if (stage >= stages) return;
+        if (!PHASED && stage >= stages) return;
         a.load(st.a, ga, stage, stride_a);
         b.load(st.b, gb, stage, stride_b);
 #pragma unroll
         for (int q = 0; q < SMOVES; ++q) {
-            const int word = tid + q * THREADS, row = word / SK, k = word % SK, at = (stage * SK + k) * 4;
-            if (row < TM) st.scale[q] = gsa.load4(row * stride_s + at);
-            else if (row < TM + TN) st.scale[q] = gsb.load4((row - TM) * stride_s + at);
+            const int word = tid + q * THREADS, row = word / SK, at = (stage * SK + word % SK) * 4;
+            if (TM * SK % 64 == 0) {                         // A's words end with a wavefront: it takes one buffer or the other
+                const bool in_a = wave * 64 + q * THREADS < TM * SK;
+                st.scale[q] = (in_a ? gsa : gsb).load4((in_a ? row : row - TM) * stride_s + at);
+            } else                                           // both, one of them behind its end
+                st.scale[q] = gsa.load4(row < TM ? row * stride_s + at : TileRows::BEHIND) | gsb.load4(row >= TM ? (row - TM) * stride_s + at : TileRows::BEHIND);
         }
     };
     const auto store = [&](const Stage &st, int stage) {
@@ -439,6 +442,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
 #pragma unroll
         for (int k = 0; k < SK; ++k) {
             if (k > 0 && t * SK + k >= p.steps) break;
+            if (PHASED && k == 0) {
+                store(next, t + 1);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             v8i fa[RT], fb[CT];
             int sa[(RT + 3) / 4], sb[(CT + 3) / 4];
 #pragma unroll
@@ -450,10 +457,15 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
 #pragma unroll
             for (int q = 0; q < (CT + 3) / 4; ++q) sb[q] = *reinterpret_cast<const int *>(&lscale[buf][k][GA + wn * CT / 4 + q][g][r][0]) >> first_b;
             if (PHASED) {
-                if (k == 0) {
-                    store(next, t + 1);
-                    load(next, t + 1 + AHEAD);
+                if (k == 0) load(next, t + 1 + AHEAD);
+                // the load path and the LDS work side by side: a load after every few fragment reads
+                constexpr int READS = RT * OpA::S1 / 64 + CT * OpB::S1 / 64 + RT / 4 + CT / 4, LOADS = OpA::MOVES + OpB::MOVES + SMOVES;
+#pragma unroll
+                for (int q = 0; q < LOADS; ++q) {
+                    __builtin_amdgcn_sched_group_barrier(0x100, READS / LOADS, 0);
+                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
                 }
+                __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
                 __builtin_amdgcn_sched_barrier(0);
                 __syncthreads();
                 __builtin_amdgcn_s_setprio(1);
@@ -526,7 +538,9 @@ template <class T> void dequantize(bts_context *ctx, const uint8_t *codes, const
 
 template <class T, int TPR, int CH> void rms_norm_launch(const NormArgs<T> &a, hipStream_t st) {
     const int rows = 256 / TPR;
-    hipLaunchKernelGGL((k_rms_norm<T, TPR, CH>), dim3((unsigned)(((long)a.n + rows - 1) / rows)), dim3(256), 0, st, a);
+    const dim3 grid((unsigned)(((long)a.n + rows - 1) / rows));
+    if (a.d % 8 == 0) hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, false>), grid, dim3(256), 0, st, a);
 }
 template <class T> void rms_norm(const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d, double eps,
                                  void *sum, int lds, void *y, int ldy, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
@@ -534,10 +548,11 @@ template <class T> void rms_norm(const void *x, int ldx, const void *residual, i
     a.x = static_cast<const T *>(x); a.residual = static_cast<const T *>(residual); a.weight = static_cast<const T *>(weight);
     a.sum = static_cast<T *>(sum); a.y = static_cast<T *>(y);
     a.ldx = ldx; a.ldr = ldr; a.lds = lds; a.ldy = ldy; a.n = n; a.d = d; a.eps = eps; a.format = format; a.codes = codes; a.scales = scales;
-    // a wavefront a row up to 2048 elements (no barrier), a workgroup beyond
+    // a wavefront a row up to 1024 elements (32768 x 512 bfloat16: 21 us against 30 with a workgroup a row, x 1024: 37 against 44), a workgroup
+    // beyond (32768 x 2048: 88 us against 95 with a wavefront a row; one row: 2.8 against 4.6)
     if (d <= 512) rms_norm_launch<T, 64, 1>(a, st);
     else if (d <= 1024) rms_norm_launch<T, 64, 2>(a, st);
-    else if (d <= 2048) rms_norm_launch<T, 64, 4>(a, st);
+    else if (d <= 2048) rms_norm_launch<T, 256, 1>(a, st);
     else if (d <= 4096) rms_norm_launch<T, 256, 2>(a, st);
     else if (d <= 8192) rms_norm_launch<T, 256, 4>(a, st);
     else rms_norm_launch<T, 256, 0>(a, st);

@@ -334,6 +334,16 @@ def test_product(bts, n, m, d, fa, fb):
         run_product(bts, n, m, d, fa, fb, out)
 
 
+# enough of them for LDS tiles of each of the small shapes
+MID = [(512, 256, 256), (3, 33000, 96), (9000, 20, 100), (1030, 1030, 100)]
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m,d", MID)
+def test_product_tiles(bts, n, m, d, fa, fb):
+    run_product(bts, n, m, d, fa, fb, "f32" if fa == fb == "e2m1" else "f16")
+
+
 @pytest.mark.parametrize("fa,fb", FMTS)
 @pytest.mark.parametrize("n,m,d", BIG)
 def test_product_big(bts, n, m, d, fa, fb):
