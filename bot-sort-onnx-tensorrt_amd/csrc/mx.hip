@@ -52,6 +52,7 @@ template <class T> struct NormArgs {
     T *sum, *y;
     long ldx, ldr, lds, ldy;
     int n, d;
+    long first;                          // the launch's first row
     double eps;
     int format;                          // -1: no quantised output
     uint8_t *codes, *scales;
@@ -70,14 +71,31 @@ template <class T, bool WHOLE> __device__ __forceinline__ void norm_load(const N
     round8<T>(h);
 }
 // 8 squares in float32 (each product of 16-bit values is exact), the row's sum in float64: the factor of a row is common to all of its
-// elements, and a factor that is off by a few roundings turns that many codes at the borders between two values
+// elements, and a factor that is off by a few roundings turns that many codes at the borders between two values.  Squares that leave
+// float32's range at either end are taken in float64.
 __device__ __forceinline__ double squares(const float (&h)[8]) {
-    return (double)(((h[0] * h[0] + h[1] * h[1]) + (h[2] * h[2] + h[3] * h[3])) + ((h[4] * h[4] + h[5] * h[5]) + (h[6] * h[6] + h[7] * h[7])));
+    const float s = ((h[0] * h[0] + h[1] * h[1]) + (h[2] * h[2] + h[3] * h[3])) + ((h[4] * h[4] + h[5] * h[5]) + (h[6] * h[6] + h[7] * h[7]));
+    if (s > 1e-30f && s < 3e38f) return (double)s;
+    double t = 0.0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) t += (double)h[e] * (double)h[e];
+    return t;
+}
+// A row's factor.  Where the row's norm passes 2^63 or stays below 2^-50, its elements are first scaled by 2^-64 or 2^64 and the factor by
+// the inverse, so that neither the factor nor the elements times the weight leave float32's range.
+struct Factor { float inv, first; };
+__device__ __forceinline__ Factor row_factor(double ss, int d, double eps) {
+    const float first = ss > 0x1p126 ? 0x1p-64f : ss < 0x1p-100 ? 0x1p64f : 1.0f;
+    return {(float)(1.0 / (sqrt(ss / (double)d + eps) * (double)first)), first};
 }
 // the normalised piece at column k: to y, and as codes (whole blocks: a block's four lanes come together)
-template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, float inv, float (&h)[8]) {
+template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, Factor f, float (&h)[8]) {
     if (k < a.d) {
         const int have = WHOLE ? 8 : a.d - k;
+        if (f.first != 1.0f) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) h[e] *= f.first;
+        }
         if (a.weight) {
             float w[8];
             load8(a.weight + k, have, w);
@@ -85,7 +103,7 @@ template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const N
             for (int e = 0; e < 8; ++e) h[e] *= w[e];             // (exact for 16-bit types: one rounding, that of the factor, follows)
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = WHOLE || e < have ? h[e] * inv : 0.0f;
+        for (int e = 0; e < 8; ++e) h[e] = WHOLE || e < have ? h[e] * f.inv : 0.0f;
         if (a.y) store8(a.y + i * a.ldy + k, have, h);
     }
     if (a.format < 0) return;
@@ -102,7 +120,7 @@ template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const N
 template <class T, int TPR, int CH, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
     __shared__ double part[4];
-    const long i = (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
+    const long i = a.first + (long)blockIdx.x * (256 / TPR) + threadIdx.x / TPR;
     const int width = (int)padded(a.d), first = (threadIdx.x % TPR) * 8;
     if (TPR == 64 && i >= a.n) return;
     float h[CH > 0 ? CH : 1][8];
@@ -135,12 +153,12 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
         __syncthreads();
         ss = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    const float inv = (float)(1.0 / sqrt(ss / (double)a.d + a.eps));
+    const Factor f = row_factor(ss, a.d, a.eps);
     if (CH > 0) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {
             const int k = first + c * TPR * 8;
-            if (k < width) norm_emit<T, WHOLE>(a, i, k, width, inv, h[c]);
+            if (k < width) norm_emit<T, WHOLE>(a, i, k, width, f, h[c]);
         }
     } else {
         for (int k = first; k < width; k += TPR * 8) {
@@ -149,7 +167,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
                 for (int e = 0; e < 8; ++e) h[0][e] = 0.0f;
             } else if (a.sum) load8(a.sum + i * a.lds + k, WHOLE ? 8 : a.d - k, h[0]);
             else norm_load<T, WHOLE>(a, i, k, h[0]);
-            norm_emit<T, WHOLE>(a, i, k, width, inv, h[0]);
+            norm_emit<T, WHOLE>(a, i, k, width, f, h[0]);
         }
     }
 }
@@ -162,6 +180,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
 struct ProductArgs {
     const uint8_t *a_codes, *a_scales, *b_codes, *b_scales;
     int n, m, steps;                     // steps of 128 elements
+    int first;                           // the launch's first tile
     float alpha;
     int floor_zero;
     void *out;
@@ -232,14 +251,13 @@ template <class T> __device__ __forceinline__ void epilogue4(const ProductArgs &
 template <int FA, int FB>
 __global__ __launch_bounds__(256) void k_mx_direct(ProductArgs p) {
     __shared__ v4f part[3][64];
-    const long tiles_n = ((long)p.m + 15) / 16, ti = blockIdx.x / tiles_n, tj = blockIdx.x % tiles_n;
+    const long tiles_n = ((long)p.m + 15) / 16, tile = (long)p.first + blockIdx.x, ti = tile / tiles_n, tj = tile % tiles_n;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, g = lane >> 4;
     const long i = min(ti * 16 + r, (long)p.n - 1), j = min(tj * 16 + r, (long)p.m - 1);      // (rows behind the last one read it; never stored)
     const uint8_t *ac = p.a_codes + i * p.steps * (FA == E2M1 ? 64 : 128), *as = p.a_scales + i * p.steps * 4 + g;
     const uint8_t *bc = p.b_codes + j * p.steps * (FB == E2M1 ? 64 : 128), *bs = p.b_scales + j * p.steps * 4 + g;
     const int per = (p.steps + 3) / 4, s0 = wave * per, s1 = min(p.steps, s0 + per);
     v4f acc = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll 2
     for (int s = s0; s < s1; ++s)
         acc = mma<FA, FB, 0, 0>(load_fragment<FB>(bc, s, g), load_fragment<FA>(ac, s, g), acc, bs[(long)s * 4], as[(long)s * 4]);
     if (wave > 0) part[wave - 1][lane] = acc;
@@ -326,11 +344,11 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
     constexpr int FRAGS = 8 / (int)sizeof(T) < CT ? 8 / (int)sizeof(T) : CT, COLS = FRAGS * 16, ROWB = COLS * (int)sizeof(T), CHUNKS = ROWB / 16;
     constexpr int ACROSS = 64 / CHUNKS < 16 ? 64 / CHUNKS : 16;                    // rows a store
     static_assert(CT % FRAGS == 0, "whole passes");
-    const int r = lane & 15, g = lane >> 4, rows = p.n - i0, cols = p.m - j0, ld = (int)p.ld * (int)sizeof(T);      // (bytes; the host's check)
-    uint8_t *const out = reinterpret_cast<uint8_t *>(static_cast<T *>(p.out) + (i0 * p.ld + j0));                   // the same in all lanes
+    const int r = lane & 15, g = lane >> 4, rows = p.n - i0, cols = p.m - j0, ld = (int)(p.ld * (long)sizeof(T));   // (bytes; the host's check)
+    uint8_t *out = reinterpret_cast<uint8_t *>(static_cast<T *>(p.out) + (i0 * p.ld + j0));                   // the same in all lanes
     const int row8 = lane / CHUNKS, at8 = row8 * ld + (lane % CHUNKS) * 16;
 #pragma unroll
-    for (int u = 0; u < RT; ++u)
+    for (int u = 0; u < RT; ++u, out += 16 * p.ld * (long)sizeof(T))
 #pragma unroll
         for (int w0 = 0; w0 < CT; w0 += FRAGS) {
             float v[FRAGS * 4];
@@ -352,14 +370,14 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
                     const int row = q * ACROSS + row8;
                     if (64 / CHUNKS > 16 && row >= 16) break;
                     const v4i x = *reinterpret_cast<const v4i *>(room + row * ROWB + ((lane % CHUNKS) ^ (row & (CHUNKS - 1))) * 16);
-                    if (u * 16 + row < rows) *reinterpret_cast<v4i *>(out + (uint32_t)(at8 + (u * 16 + q * ACROSS) * ld + w0 * 16 * (int)sizeof(T))) = x;
+                    if (u * 16 + row < rows) *reinterpret_cast<v4i *>(out + (uint32_t)(at8 + q * ACROSS * ld + w0 * 16 * (int)sizeof(T))) = x;
                 }
             } else {
 #pragma unroll 4
                 for (int q = 0; q < 16 * COLS / 64; ++q) {
                     const int row = q * (64 / COLS) + lane / COLS, col = lane % COLS, at = col * (int)sizeof(T);
                     const T x = *reinterpret_cast<const T *>(room + row * ROWB + ((at / 16) ^ (row & (CHUNKS - 1))) * 16 + at % 16);
-                    if (u * 16 + row < rows && w0 * 16 + col < cols) *reinterpret_cast<T *>(out + (uint32_t)((u * 16 + row) * ld + (w0 * 16 + col) * (int)sizeof(T))) = x;
+                    if (u * 16 + row < rows && w0 * 16 + col < cols) *reinterpret_cast<T *>(out + (uint32_t)(row * ld + (w0 * 16 + col) * (int)sizeof(T))) = x;
                 }
             }
             __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
@@ -390,7 +408,7 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     const int wm = wave / WN, wn = wave % WN;
     const int first_a = 8 * (wm * RT % 4), first_b = 8 * (wn * CT % 4);      // where a wavefront's fragments begin in their group's words
     int tm, tn;
-    tile_of(blockIdx.x, (p.n + TM - 1) / TM, (p.m + TN - 1) / TN, tm, tn);
+    tile_of(p.first + (int)blockIdx.x, (p.n + TM - 1) / TM, (p.m + TN - 1) / TN, tm, tn);
 
     const int stride_a = p.steps * OpA::S1, stride_b = p.steps * OpB::S1, stride_s = p.steps * 4, stages = (p.steps + SK - 1) / SK;
     const TileRows ga(p.a_codes, tm * TM, p.n, TM, stride_a), gb(p.b_codes, tn * TN, p.m, TN, stride_b);
@@ -516,6 +534,7 @@ bool known_format(int f) { return f == BTS_MX_E2M1 || f == BTS_MX_E4M3; }
 bool known_dtype(int t) { return t == BTS_F32 || t == BTS_F16 || t == BTS_BF16; }
 size_t dtype_bytes(int t) { return t == BTS_F32 ? 4 : 2; }
 bool aligned(const void *p, size_t to) { return (uintptr_t)p % to == 0; }
+constexpr int MOST_WIDE = 1 << 30;                             // a row's elements: its columns, padded and a stride further, are ints
 constexpr long MOST_PIECES = 0xffffffffl - (1 << 24);          // 128-element pieces a call takes (the grid's stride is added in 32 bits)
 long pieces(int n, int d) { return (long)n * (padded(d) / MX_ROW); }
 dim3 piece_grid(const bts_context *ctx, long pieces) {
@@ -536,11 +555,17 @@ template <class T> void dequantize(bts_context *ctx, const uint8_t *codes, const
     else hipLaunchKernelGGL((k_mx_dequantize<T, E4M3>), piece_grid(ctx, all), dim3(256), 0, st, codes, scales, all, row, d, to, (long)ldo);
 }
 
-template <class T, int TPR, int CH> void rms_norm_launch(const NormArgs<T> &a, hipStream_t st) {
+// A launch's threads have to number below 2^32: what takes more workgroups than this (a multiple of the 8 XCDs) goes out in several.
+constexpr long RUN = 1L << 20;
+
+template <class T, int TPR, int CH> void rms_norm_launch(NormArgs<T> a, hipStream_t st) {
     const int rows = 256 / TPR;
-    const dim3 grid((unsigned)(((long)a.n + rows - 1) / rows));
-    if (a.d % 8 == 0) hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, true>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, false>), grid, dim3(256), 0, st, a);
+    for (a.first = 0; a.first < a.n; a.first += RUN * rows) {
+        const long blocks = (a.n - a.first + rows - 1) / rows;
+        const dim3 grid((unsigned)(blocks < RUN ? blocks : RUN));
+        if (a.d % 8 == 0) hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_rms_norm<T, TPR, CH, false>), grid, dim3(256), 0, st, a);
+    }
 }
 template <class T> void rms_norm(const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d, double eps,
                                  void *sum, int lds, void *y, int ldy, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
@@ -558,9 +583,16 @@ template <class T> void rms_norm(const void *x, int ldx, const void *residual, i
     else rms_norm_launch<T, 256, 0>(a, st);
 }
 
-template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> void tile_launch(const ProductArgs &p, hipStream_t st) {
-    const long tiles = (((long)p.n + TM - 1) / TM) * (((long)p.m + TN - 1) / TN);
-    hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK, AHEAD>), dim3((unsigned)tiles), dim3(64 * WM * WN), 0, st, p);
+// launch(grid) of `tiles` workgroups
+template <class Launch> void in_runs(ProductArgs &p, long tiles, Launch launch) {
+    for (long first = 0; first < tiles; first += RUN) {
+        p.first = (int)first;
+        launch(dim3((unsigned)(tiles - first < RUN ? tiles - first : RUN)));
+    }
+}
+template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> void tile_launch(ProductArgs p, hipStream_t st) {
+    in_runs(p, (((long)p.n + TM - 1) / TM) * (((long)p.m + TN - 1) / TN),
+            [&](dim3 grid) { hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK, AHEAD>), grid, dim3(64 * WM * WN), 0, st, p); });
 }
 // Which kernel: by how many workgroups the sizes make of the chip, measured at d = 2048 unless said otherwise (us, E4M3 x E2M1).
 //  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 439 against
@@ -569,18 +601,28 @@ template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> voi
 //  - 64 x 64 tiles from one a CU on (48 x 65536: 19; 1000 x 1000 x 1000: 6.6 against 11), below that 16 x 64 ones (200 x 2000 x 1024: 4.9 against
 //    6.0), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.5 against 18).
 //  - 16 x 16 tiles with the row split where there are fewer than two of them a CU (1 x 2000: 3.6 against 5.4).
-template <int FA, int FB> int product(bts_context *ctx, const ProductArgs &p, hipStream_t st) {
+template <int FA, int FB> int product(bts_context *ctx, ProductArgs p, hipStream_t st) {
     const auto tiles = [&](long a, long b) { return ((p.n + a - 1) / a) * ((p.m + b - 1) / b); };
     const long cus = ctx->n_cu, t256 = tiles(256, 256), t128 = tiles(128, 128), most = 1L << 31;
     BTS_REQUIRE(tiles(16, 16) < most, "n * m: too many tiles for one launch");
     constexpr int SK = FA == E2M1 && FB == E2M1 ? 2 : 1;      // 128 bytes a row and stage
     constexpr bool BIG = FA == E2M1 || FB == E2M1;
-    // 32-bit offsets inside a tile: 256 rows of codes, 128 rows of the output
-    const bool fits = (long)p.steps * 128 * 256 < most && p.ld * 4 * 128 < most && p.n < most - 256 && p.m < most - 256;
-    if (!fits || tiles(16, 16) < 2 * cus) hipLaunchKernelGGL((k_mx_direct<FA, FB>), dim3((unsigned)tiles(16, 16)), dim3(256), 0, st, p);
-    else if (p.n <= 32) tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
+    // 32-bit offsets inside a tile: 256 rows of codes, 16 rows of the output
+    const bool fits = (long)p.steps * 128 * 256 < most && p.ld * 4 * 16 < most && p.n < most - 256 && p.m < most - 256;
+    if (!fits || tiles(16, 16) < 2 * cus) {
+        in_runs(p, tiles(16, 16), [&](dim3 grid) { hipLaunchKernelGGL((k_mx_direct<FA, FB>), grid, dim3(256), 0, st, p); });
+        BTS_LAUNCH_CHECK();
+        return BTS_OK;
+    }
+    if constexpr (BIG) {
+        if ((t256 + cus - 1) / cus * cus * 4 * 2 <= t128 * 3) {
+            tile_launch<FA, FB, 256, 256, FA == E2M1 ? 2 : 4, FA == E2M1 ? 4 : 2, 1, 1>(p, st);
+            BTS_LAUNCH_CHECK();
+            return BTS_OK;
+        }
+    }
+    if (p.n <= 32) tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
     else if (p.m <= 32) tile_launch<FA, FB, 64, 16, 4, 1, 2, 2>(p, st);
-    else if (BIG && (t256 + cus - 1) / cus * cus * 4 * 2 <= t128 * 3) tile_launch<FA, FB, 256, BIG ? 256 : 128, FA == E2M1 ? 2 : 4, FA == E2M1 ? 4 : 2, 1, 1>(p, st);
     else if (t128 >= 2 * cus) tile_launch<FA, FB, 128, 128, 2, 2, SK, 2>(p, st);
     else if (tiles(64, 64) >= cus) tile_launch<FA, FB, 64, 64, 1, 4, SK, 2>(p, st);
     else tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
@@ -594,7 +636,7 @@ extern "C" {
 
 int bts_mx_row_bytes(int format, int d, int64_t *code_bytes, int64_t *scale_bytes) {
     BTS_REQUIRE(known_format(format), "unknown format");
-    BTS_REQUIRE(d > 0 && code_bytes && scale_bytes, "d, code_bytes, scale_bytes");
+    BTS_REQUIRE(d > 0 && d <= MOST_WIDE && code_bytes && scale_bytes, "d (1 .. 2^30), code_bytes, scale_bytes");
     *code_bytes = mx::code_bytes(format, d);
     *scale_bytes = mx::scale_bytes(d);
     return BTS_OK;
@@ -602,7 +644,7 @@ int bts_mx_row_bytes(int format, int d, int64_t *code_bytes, int64_t *scale_byte
 
 int bts_mx_quantize(bts_context *ctx, const void *x, int x_dtype, int ldx, int n, int d, int format, uint8_t *codes, uint8_t *scales,
                     bts_stream stream) {
-    BTS_REQUIRE(ctx && n >= 0 && d > 0 && ldx >= d, "ctx, n, d, ldx < d");
+    BTS_REQUIRE(ctx && n >= 0 && d > 0 && d <= MOST_WIDE && ldx >= d, "ctx, n, d (1 .. 2^30), ldx < d");
     BTS_REQUIRE(known_format(format) && known_dtype(x_dtype), "unknown format / type");
     BTS_ON_DEVICE(ctx);
     if (n == 0) return BTS_OK;
@@ -619,7 +661,7 @@ int bts_mx_quantize(bts_context *ctx, const void *x, int x_dtype, int ldx, int n
 
 int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *scales, int format, int n, int d, void *out, int out_dtype,
                       int ldo, bts_stream stream) {
-    BTS_REQUIRE(ctx && n >= 0 && d > 0 && ldo >= d, "ctx, n, d, ldo < d");
+    BTS_REQUIRE(ctx && n >= 0 && d > 0 && d <= MOST_WIDE && ldo >= d, "ctx, n, d (1 .. 2^30), ldo < d");
     BTS_REQUIRE(known_format(format) && known_dtype(out_dtype), "unknown format / type");
     BTS_ON_DEVICE(ctx);
     if (n == 0) return BTS_OK;
@@ -636,7 +678,7 @@ int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *sca
 
 int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void *residual, int ldr, const void *weight, int n, int d,
                  double eps, void *sum, int lds, void *y, int ldy, int format, uint8_t *codes, uint8_t *scales, bts_stream stream) {
-    BTS_REQUIRE(ctx && n >= 0 && d > 0 && ldx >= d, "ctx, n, d, ldx < d");
+    BTS_REQUIRE(ctx && n >= 0 && d > 0 && d <= MOST_WIDE && ldx >= d, "ctx, n, d (1 .. 2^30), ldx < d");
     BTS_REQUIRE(known_dtype(dtype), "unknown type");
     BTS_REQUIRE((float)eps > 0.0f && (float)eps <= 3.0e38f, "eps must be a positive finite float32");
     BTS_REQUIRE(!residual || ldr >= d, "ldr < d");
@@ -667,7 +709,7 @@ int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void
 int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_scales, int a_format, int n, const uint8_t *b_codes,
                    const uint8_t *b_scales, int b_format, int m, int d, double alpha, int floor_zero, void *out, int out_dtype, int ld,
                    bts_stream stream) {
-    BTS_REQUIRE(ctx && n >= 0 && m >= 0 && d > 0 && ld >= m, "ctx, n, m, d, ld < m");
+    BTS_REQUIRE(ctx && n >= 0 && m >= 0 && d > 0 && d <= MOST_WIDE && ld >= m, "ctx, n, m, d (1 .. 2^30), ld < m");
     BTS_REQUIRE(known_format(a_format) && known_format(b_format) && known_dtype(out_dtype), "unknown format / type");
     BTS_REQUIRE(out_dtype != BTS_F32 || (a_format == E2M1 && b_format == E2M1),
                 "a float32 output needs two E2M1 operands (products with an E4M3 operand carry about 16 bits)");

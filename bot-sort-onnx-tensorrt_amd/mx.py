@@ -15,6 +15,7 @@ _DTYPES = {}                            # enum bts_dtype
 _raw_stream = None
 _FORMATS = {"e2m1": 0, "e4m3": 1}       # enum bts_mx_format
 _ROW, _BLOCK = 128, 32                  # elements a row is padded to; elements per scale
+_MOST = 0x7fffffff                      # rows and row strides are C ints
 
 
 def _init():
@@ -42,6 +43,14 @@ def _format_code(fmt):
     return code
 
 
+def _width(d):
+    """elements of a padded row"""
+    d = int(d)
+    if not 0 < d <= 1 << 30:
+        raise _lib.BtsError("mx rows: d must lie in 1 .. 2^30, got %d" % d)
+    return (d + _ROW - 1) // _ROW * _ROW
+
+
 def _rows2d(t, name, like=None):
     """A device matrix with unit column stride -> (pointer, row stride in elements)."""
     if not t.is_cuda:
@@ -54,6 +63,8 @@ def _rows2d(t, name, like=None):
         ld = max(d, 1)
     if (unit != 1 and d > 1) or ld < d:
         raise _lib.BtsError("%s: the elements of a row must be adjacent and rows may not overlap (strides %s): call .contiguous()" % (name, t.stride()))
+    if n > _MOST or ld > _MOST:
+        raise _lib.BtsError("%s: at most 2^31 - 1 rows, and elements between them" % name)
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
         raise _lib.BtsError("%s: shape, type and device of x expected (%s %s %s)" % (name, tuple(like.shape), like.dtype, like.device))
     return t.data_ptr(), ld
@@ -70,6 +81,7 @@ def _call(device):
 def mx_row_bytes(fmt: str, d: int) -> "tuple[int, int]":
     """(code bytes, scale bytes) of one row of d elements."""
     c, s = ctypes.c_int64(), ctypes.c_int64()
+    _width(d)
     _lib.check(_lib.load().bts_mx_row_bytes(_format_code(fmt), int(d), ctypes.byref(c), ctypes.byref(s)))
     return c.value, s.value
 
@@ -84,11 +96,8 @@ class MxRows:
         if torch is None:
             _init()
         self._code = _format_code(fmt)
-        d = int(d)
-        if d <= 0:
-            raise _lib.BtsError("MxRows: d must be positive")
-        wide = (d + _ROW - 1) // _ROW * _ROW
-        n = codes.shape[0] if codes.dim() == 2 else -1
+        d, wide = int(d), _width(d)
+        n = codes.shape[0] if codes.dim() == 2 and codes.shape[0] <= _MOST else -1
         if (codes.dtype != torch.uint8 or scales.dtype != torch.uint8 or codes.shape != (n, wide // 2 if fmt == "e2m1" else wide)
                 or scales.shape != (n, wide // _BLOCK)):
             raise _lib.BtsError("MxRows: uint8 codes [n, %d] and scales [n, %d] expected for d = %d in %s, got %s %s" % (
@@ -117,9 +126,9 @@ class MxRows:
         """Room for n rows."""
         if torch is None:
             _init()
-        code, wide = _format_code(fmt), (int(d) + _ROW - 1) // _ROW * _ROW
-        if wide <= 0:
-            raise _lib.BtsError("MxRows: d must be positive")
+        code, wide = _format_code(fmt), _width(d)
+        if not 0 <= n <= _MOST:
+            raise _lib.BtsError("MxRows: 0 .. 2^31 - 1 rows, got %d" % n)
         device = torch.device(device)
         return cls._of(torch.empty((n, wide // 2 if code == 0 else wide), dtype=torch.uint8, device=device),
                        torch.empty((n, wide // _BLOCK), dtype=torch.uint8, device=device), int(d), fmt, code)

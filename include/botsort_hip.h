@@ -169,7 +169,7 @@ int bts_feature_renorm(bts_context *ctx, float *feats, const int32_t *idx, int k
  * zero-padded to a multiple of 128 elements; rows follow each other without gaps.  codes: 16-byte, scales: 4-byte aligned.
  * Quantisation (OCP microscaling formats): s = 127 + clamp(floor(log2(max |v|)) - emax, -127, 127), emax = 2 (E2M1) / 8 (E4M3),
  * elements v / 2^(s - 127) rounded to nearest even, saturating.  A block with an infinity or a NaN in it becomes NaN.
- * Types of x / out / y: BTS_F32, BTS_F16 or BTS_BF16 (enum bts_dtype); row strides (ld*) are in elements, >= d. */
+ * Types of x / out / y: BTS_F32, BTS_F16 or BTS_BF16 (enum bts_dtype); row strides (ld*) are in elements, >= d; d <= 2^30. */
 enum bts_mx_format { BTS_MX_E2M1 = 0, BTS_MX_E4M3 = 1 };
 
 /* Bytes of one row's codes and scales (host-only). */
@@ -187,7 +187,7 @@ int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *sca
  *   h = x + residual, rounded to `dtype` (h = x without a residual);   v = h / sqrt(mean(h^2) + eps) * weight
  * sum (nullable) = h; y (nullable) = v in `dtype`; codes / scales (both nullable) = v in `format`, quantised from float32.
  * residual[n,d] and weight[d] are nullable, all of x's type.  sum and y may be x or residual themselves (same row stride), not
- * each other.  The mean is taken in float32: rows whose sum of squares passes its range are outside.  eps > 0. */
+ * each other.  eps: a positive finite float32. */
 int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void *residual, int ldr,
                  const void *weight, int n, int d, double eps, void *sum, int lds, void *y, int ldy,
                  int format, uint8_t *codes, uint8_t *scales, bts_stream stream);

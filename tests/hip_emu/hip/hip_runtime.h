@@ -266,18 +266,6 @@ template <class T> static inline T emu_buffer_load(__amdgpu_buffer_rsrc_t r, int
 #define __builtin_amdgcn_raw_buffer_load_b128(r, at, base, aux) emu_buffer_load<emu_u32x4>((r), (at) + (base))
 #define __builtin_amdgcn_raw_buffer_load_b32(r, at, base, aux) emu_buffer_load<unsigned>((r), (at) + (base))
 #define __builtin_amdgcn_make_buffer_rsrc(p, stride, size, flags) emu_make_rsrc((p), (size))
-// ... and the same from a buffer to LDS: lane l's bytes land at base + size l, asynchronously like global_load_lds below
-static inline void emu_buffer_load_lds(__amdgpu_buffer_rsrc_t r, void *lds_base, int size, int at);
-#define __builtin_amdgcn_raw_ptr_buffer_load_lds(r, lds, size, at, base, off, aux) emu_buffer_load_lds((r), (void *)(lds), (size), (at) + (base) + (off))
-static inline unsigned emu_perm(unsigned hi, unsigned lo, unsigned sel) {
-    unsigned out = 0;
-    for (int k = 0; k < 4; ++k) {
-        const unsigned s = (sel >> (8 * k)) & 255;
-        if (s < 8) out |= (((s < 4 ? lo : hi) >> (8 * (s & 3))) & 255u) << (8 * k);      /* 12: a zero byte */
-    }
-    return out;
-}
-#define __builtin_amdgcn_perm(hi, lo, sel) emu_perm((hi), (lo), (sel))
 // conversions of two codes back: value * 2^(exponent field of the scale - 127), rounded once to the output's type
 typedef float emu_f32x2 __attribute__((ext_vector_type(2)));
 static inline double emu_scaled(int fmt, unsigned code, float scale) {
@@ -331,11 +319,6 @@ void lds_dma_check(const void *p, int n, const char *what);    // an LDS read / 
 }
 static inline void emu_global_load_lds(const void *g, void *lds_base, int size) {
     emu::lds_dma_issue(g, (char *)lds_base + (size_t)(emu::tid_x() & 63) * (size_t)size, size);
-}
-static inline void emu_buffer_load_lds(__amdgpu_buffer_rsrc_t r, void *lds_base, int size, int at) {
-    static const char zeros[16] = {0};
-    const bool inside = (uint64_t)(unsigned)at + (unsigned)size <= r.size;
-    emu::lds_dma_issue(inside ? (const void *)(r.base + (unsigned)at) : (const void *)zeros, (char *)lds_base + (size_t)(emu::tid_x() & 63) * (size_t)size, size);
 }
 #define __builtin_amdgcn_global_load_lds(g, l, size, off, aux) emu_global_load_lds((const void *)(g), (void *)(l), (size))
 

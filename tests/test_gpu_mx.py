@@ -262,6 +262,38 @@ def test_rms_norm_in_place(bts, d):
     assert torch.equal(xd.cpu(), y0.cpu())
 
 
+@pytest.mark.parametrize("d", [40, 1500, 9000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rms_norm_at_the_ends_of_the_range(bts, d, dtype):
+    """rows whose squares, or whose products with the weight, leave float32 in either direction"""
+    t, r = DTYPES[dtype], np.random.default_rng(d)
+    e = np.array([127, 126, 100, 64, 62, -40, -60, -90, -110])                      # (normal values: the smallest are 2^-118)
+    v = (1 + r.random((len(e), d))) * np.exp2(e[:, None] - (r.integers(0, 9, (len(e), d)) if dtype == "f32" else 0)) * r.choice([-1, 1], (len(e), d))
+    x = torch.from_numpy(np.clip(v, -float(torch.finfo(t).max), float(torch.finfo(t).max))).to(t)
+    w = torch.from_numpy(r.choice([0.25, 3.0, 40.0], d)).to(t)
+    for eps in (1e-6, 1e-38):
+        y = torch.empty_like(x).cuda()
+        q, h = bts.rms_norm_mx(x.cuda(), weight=w.cuda(), eps=eps, y_out=y)
+        _, want = norm_ref(x, None, w, eps)
+        delta = norm_delta(d)
+        tol = (delta + HALF[dtype] * (1 + delta)) * np.abs(want) + float(torch.finfo(t).smallest_normal) * HALF[dtype]
+        assert (np.abs(y.cpu().double().numpy() - want) <= tol).all()
+        check_quantized(want, *host(q), "e4m3", d, delta)
+
+
+# more rows than one launch's workgroups, 4 rows each up to 1024 elements
+@pytest.mark.parametrize("n,d", [(4 * 2 ** 20 + 5, 8), (2 ** 20 + 3, 1032)])
+def test_rms_norm_big_row_counts(bts, n, d):
+    x = torch.ones((n, d), dtype=torch.float16, device="cuda")
+    x[-9:] = torch.from_numpy(np.random.default_rng(n).standard_normal((9, d))).half().cuda()
+    y = torch.zeros_like(x)
+    bts.rms_norm_mx(x, fmt=None, y_out=y)
+    assert (y[:-9] == 1).all()                                                      # 1 / sqrt(1 + 1e-6) rounds to 1
+    _, v = norm_ref(x[-9:].cpu(), None, None, 1e-6)
+    delta = norm_delta(d)
+    assert (np.abs(y[-9:].cpu().double().numpy() - v) <= (delta + HALF["f16"] * (1 + delta)) * np.abs(v) + 2.0 ** -25).all()
+
+
 def test_rms_norm_zero_and_non_finite_rows(bts):
     x = torch.ones((5, 300))
     x[1] = 0; x[2, 7] = float("inf"); x[3, 70] = float("nan")
@@ -348,6 +380,38 @@ def test_product_tiles(bts, n, m, d, fa, fb):
 @pytest.mark.parametrize("n,m,d", BIG)
 def test_product_big(bts, n, m, d, fa, fb):
     run_product(bts, n, m, d, fa, fb, "f32" if fa == fb == "e2m1" else "bf16")
+
+
+def test_product_big_row_counts(bts):
+    """more tiles than one launch's workgroups; an output whose row stride is wide"""
+    m, at = 2 ** 26 + 700, [0, 5, 2 ** 26 - 1, 2 ** 26, 2 ** 26 + 63, 2 ** 26 + 64, 2 ** 26 + 699]
+    one, row = feature_rows(2, 128, 1), feature_rows(len(at), 128, 2)
+    a, ra = rows_of(bts, one, "e2m1")
+    few, rb = rows_of(bts, row, "e2m1")
+    b = bts.MxRows(few.codes[:1].repeat(m, 1), few.scales[:1].repeat(m, 1), 128, "e2m1")
+    for k, i in enumerate(at):
+        b.codes[i], b.scales[i] = few.codes[k], few.scales[k]
+    got = bts.mx_product(a, b, dtype=torch.bfloat16)
+    want = ra @ rb.T
+    tol = product_bound(ra, rb, "bf16", want, ("e2m1", "e2m1"))
+    assert (np.abs(got[:, at].cpu().double().numpy() - want) <= tol).all()
+    rest = torch.ones(m, dtype=torch.bool)
+    rest[at] = False
+    assert (got.cpu()[:, rest] == got[:, :1].cpu()).all()
+    got = bts.mx_product(b, a, dtype=torch.bfloat16)
+    assert (np.abs(got[at].cpu().double().numpy() - want.T) <= tol.T).all() and (got.cpu()[rest] == got[:1].cpu()).all()
+
+
+@pytest.mark.parametrize("n,cols", [(70, 5_000_000), (40, 40_000_000)])
+def test_product_big_row_strides(bts, n, cols):
+    """a block of a matrix whose rows lie far apart: 64-bit places between the rows of one tile"""
+    out = torch.zeros((n, cols), dtype=torch.bfloat16, device="cuda")
+    a, ra = rows_of(bts, feature_rows(n, 200, 1), "e4m3")
+    b, rb = rows_of(bts, feature_rows(3000, 200, 2), "e2m1")
+    got = bts.mx_product(a, b, out=out[:, 1000:4000]).cpu().double().numpy()
+    want = ra @ rb.T
+    assert (np.abs(got - want) <= product_bound(ra, rb, "bf16", want, ("e4m3", "e2m1"))).all()
+    assert (out[:, :1000] == 0).all() and (out[:, 4000:] == 0).all()
 
 
 @pytest.mark.parametrize("fa,fb", FMTS)
@@ -471,6 +535,11 @@ def test_refusals(bts):
         lambda: bts.mx_product(q, q, out=torch.empty((4, 4)).cuda(), dtype=torch.float16),
         lambda: bts.mx_product(q, q, out=torch.empty((4, 4)).cuda().t()),
         lambda: bts.mx_row_bytes("e2m1", 0),
+        lambda: bts.mx_row_bytes("e2m1", 2 ** 30 + 1),
+        lambda: bts.mx_row_bytes("e2m1", 2 ** 32 + 5),
+        lambda: bts.MxRows.empty(1, 2 ** 32 + 5, "e2m1"),
+        lambda: bts.MxRows.empty(2 ** 31, 1, "e2m1"),
+        lambda: bts.MxRows.empty(-1, 1, "e2m1"),
     ]
     for k, f in enumerate(bad):
         with pytest.raises(bts.BtsError):
