@@ -290,6 +290,16 @@ struct TileRows {
     __device__ __forceinline__ uint32_t load4(int at) const { return __builtin_amdgcn_raw_buffer_load_b32(rsrc, at, 0, 0); }
 };
 
+// Lane l has the four scale bytes of row l; after this it has byte l >> 4 of the rows l & 15, that + 16, + 32 and + 48: those of its elements
+// in four fragments.  (A 4 x 4 transposition of bytes over lanes 16 apart, so that they go to LDS a word at a time instead of four bytes:
+// 10000 x 2000 x 8192 took 132 us instead of 138.)
+__device__ __forceinline__ uint32_t transpose_bytes(uint32_t w, int lane) {
+    const auto far = __builtin_amdgcn_permlane32_swap(w, w, false, false);        // [0]: the word of the lane's pair with bit 5 clear, [1]: set
+    w = __builtin_amdgcn_perm(far[1], far[0], lane & 32 ? 0x07060302u : 0x05040100u);
+    const auto near = __builtin_amdgcn_permlane16_swap(w, w, false, false);       // ... bit 4
+    return __builtin_amdgcn_perm(near[1], near[0], lane & 16 ? 0x07030501u : 0x06020400u);
+}
+
 // One operand of a stage: ROWS rows of SK instruction depths, moved by THREADS threads.  A row of a stage is C 16-byte chunks; chunk c of
 // row r lies at c ^ swizzle(r), so that the 16 lanes that an LDS read serves at a time -- 16 rows of one chunk, or 8 rows of each of two
 // neighbouring chunks -- are in 16 different 16-byte bank groups (no bank conflict counted; 4 cycles a read with rows / 4 in the
@@ -302,11 +312,12 @@ template <int FMT, int ROWS, int THREADS, int SK> struct Operand {
     static constexpr int BYTES = ROWS * S;
     static_assert((MOVES * THREADS == ROWS * C || MOVES == 1) && MOVES % PERIOD == 0, "even staging");
     static __device__ __forceinline__ int swizzle(int row) { return (C >= 16 ? row : C == 8 ? row / 2 : -(row / 4)) & (C >= 16 ? 15 : C - 1); }
-    int from, to[PERIOD], frag[SK][S1 / 64];
+    int from, depth, to[PERIOD], frag[SK][S1 / 64];
     struct Regs { v4i chunk[MOVES]; };
     __device__ __forceinline__ void init(int tid, int first_row, int r, int g, int stride) {
         const int row = tid / C, c = tid % C;
         from = row * stride + c * 16;
+        depth = c / (S1 / 16);
 #pragma unroll
         for (int q = 0; q < PERIOD; ++q) to[q] = (row + q * STEP) * S + (c ^ swizzle(row + q * STEP)) * 16;
 #pragma unroll
@@ -314,9 +325,11 @@ template <int FMT, int ROWS, int THREADS, int SK> struct Operand {
 #pragma unroll
             for (int h = 0; h < S1 / 64; ++h) frag[k][h] = (first_row + r) * S + ((k * (S1 / 16) + 4 * h + g) ^ swizzle(r)) * 16;
     }
-    __device__ __forceinline__ void load(Regs &x, const TileRows &rows, int stage, int stride) const {
+    // depths behind the row's end are zeros (the buffer goes on there with the next row)
+    __device__ __forceinline__ void load(Regs &x, const TileRows &rows, int stage, int stride, int steps) const {
+        const uint32_t at = stage * SK + depth >= steps ? TileRows::BEHIND : from + stage * S;
 #pragma unroll
-        for (int q = 0; q < MOVES; ++q) x.chunk[q] = rows.load16(from + q * STEP * stride + stage * S);
+        for (int q = 0; q < MOVES; ++q) x.chunk[q] = rows.load16((int)(at + q * STEP * stride));
     }
     __device__ __forceinline__ void store(const Regs &x, uint8_t *image) const {
 #pragma unroll
@@ -390,7 +403,11 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
 // (Fragments straight from memory would be 16 rows x 64 bytes a load with the lanes of a row 16 apart: a quarter of the load path's rate.)
 // With 8 wavefronts (two a SIMD) the second four run one phase behind the first: while one of a SIMD's two wavefronts multiplies, the
 // other fetches its fragments, stores the next stage and issues the loads of the one after; barriers keep the two in step.  With 4
-// wavefronts a stage has one barrier, and the workgroups of a CU take turns.
+// wavefronts a stage has one barrier, a depth's fragments are read while the one before it is multiplied (1000 x 1000 x 1000: 5.2 us
+// against 6.6 with both in turn), and the workgroups of a CU overlap.
+// What bounds it (128 x 128, E2M1 x E2M1, 10240 x 2048 x 8192, 128 us): the output and the instructions alone take 80, the writes to LDS 29
+// more, the loads behind them 25; fragment reads cost nothing.  A round of tiles computes and then stores together, so the output of
+// 10000 x 2000 float32 (17 us) comes on top of the loop (14 us per 1024 elements of depth).
 template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     constexpr int THREADS = 64 * WM * WN, RT = TM / WM / 16, CT = TN / WN / 16;
@@ -399,11 +416,11 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     typedef Operand<FB, TN, THREADS, SK> OpB;
     static_assert((RT % 4 == 0 || TM <= 64) && (CT % 4 == 0 || TN <= 64), "scale bytes come four fragments to a word");
     constexpr int GA = (TM + 63) / 64, GB = (TN + 63) / 64;  // groups of 64 rows = four fragments
-    constexpr int WORDS = (TM + TN) * SK, SMOVES = (WORDS + THREADS - 1) / THREADS;
+    constexpr int SMOVES = (GA + GB + WM * WN - 1) / (WM * WN);      // groups whose scale bytes a wavefront moves
     constexpr int B_AT = 2 * OpA::BYTES, IMAGES = B_AT + 2 * OpB::BYTES, ROOM = WM * WN * 2048;      // A's two images, then B's
     __shared__ __attribute__((aligned(1024))) uint8_t image[IMAGES > ROOM ? IMAGES : ROOM];
-    // scale bytes: [group][lane group][row of a fragment][fragment], so that a lane's four are one word
-    __shared__ __attribute__((aligned(16))) uint8_t lscale[2][SK][GA + GB][4][16][4];
+    // scale bytes: lane l's word holds those of four fragments
+    __shared__ uint32_t lscale[2][SK][GA + GB][64];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r = lane & 15, g = lane >> 4;
     const int wm = wave / WN, wn = wave % WN;
     const int first_a = 8 * (wm * RT % 4), first_b = 8 * (wn * CT % 4);      // where a wavefront's fragments begin in their group's words
@@ -417,93 +434,57 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     OpB b;
     a.init(tid, wm * RT * 16, r, g, stride_a);
     b.init(tid, wn * CT * 16, r, g, stride_b);
-    // (Depths behind the row's end load the next row's beginning, or zeros; they are not multiplied.  Nor is the one stage behind it that the
-    // phased form loads rather than branch between its reads.)
-    struct Stage { typename OpA::Regs a; typename OpB::Regs b; uint32_t scale[SMOVES]; };
+    // (No branches around loads and stores: where the paths meet, the compiler would wait for all loads in flight.  Stages and depths behind
+    // the row's end are zeros.)
+    struct Stage { typename OpA::Regs a; typename OpB::Regs b; uint32_t scale[SMOVES][SK]; };
     const auto load = [&](Stage &st, int stage) {
-        if (!PHASED && stage >= stages) return;
-        a.load(st.a, ga, stage, stride_a);
-        b.load(st.b, gb, stage, stride_b);
+        a.load(st.a, ga, stage, stride_a, p.steps);
+        b.load(st.b, gb, stage, stride_b, p.steps);
+        // a lane takes one row's scale bytes, a word a depth
 #pragma unroll
         for (int q = 0; q < SMOVES; ++q) {
-            const int word = tid + q * THREADS, row = word / SK, at = (stage * SK + word % SK) * 4;
-            if (TM * SK % 64 == 0) {                         // A's words end with a wavefront: it takes one buffer or the other
-                const bool in_a = wave * 64 + q * THREADS < TM * SK;
-                st.scale[q] = (in_a ? gsa : gsb).load4((in_a ? row : row - TM) * stride_s + at);
-            } else                                           // both, one of them behind its end
-                st.scale[q] = gsa.load4(row < TM ? row * stride_s + at : TileRows::BEHIND) | gsb.load4(row >= TM ? (row - TM) * stride_s + at : TileRows::BEHIND);
+            const int group = wave + q * WM * WN, row = (group < GA ? group : group - GA) * 64 + lane;
+            const uint32_t at = stage >= stages || group >= GA + GB ? TileRows::BEHIND : row * stride_s + stage * SK * 4;
+            const TileRows &rows = group < GA ? gsa : gsb;
+#pragma unroll
+            for (int k = 0; k < SK; ++k) st.scale[q][k] = rows.load4((int)(at + 4 * k));
         }
     };
     const auto store = [&](const Stage &st, int stage) {
-        if (stage >= stages) return;
         const int buf = stage & 1;
         a.store(st.a, image + buf * OpA::BYTES);
         b.store(st.b, image + B_AT + buf * OpB::BYTES);
 #pragma unroll
-        for (int q = 0; q < SMOVES; ++q) {
-            const int word = tid + q * THREADS, k = word % SK, row = word / SK < TM ? word / SK : word / SK - TM, base = word / SK < TM ? 0 : GA;
-            if (word < WORDS) {
-                uint8_t *to = &lscale[buf][k][base + (row >> 6)][0][row & 15][(row >> 4) & 3];
+        for (int q = 0; q < SMOVES; ++q)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) to[64 * e] = (uint8_t)(st.scale[q] >> (8 * e));
+            for (int k = 0; k < SK; ++k) {
+                const int group = wave + q * WM * WN;
+                const uint32_t word = transpose_bytes(stage * SK + k < p.steps ? st.scale[q][k] : 0, lane);
+                if ((GA + GB) % (WM * WN) == 0 || group < GA + GB) lscale[buf][k][group][lane] = word;
             }
-        }
     };
     v4f acc[RT][CT];
 #pragma unroll
     for (int u = 0; u < RT; ++u)
 #pragma unroll
         for (int w = 0; w < CT; ++w) acc[u][w] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-    // stage t, the next one in `next`
-    const auto step = [&](int t, Stage &next) {
+    struct Fragments { v8i a[RT], b[CT]; int sa[(RT + 3) / 4], sb[(CT + 3) / 4]; };
+    const auto read = [&](Fragments &f, int t, int k) {      // depth k of stage t
         const int buf = t & 1;
 #pragma unroll
-        for (int k = 0; k < SK; ++k) {
-            if (k > 0 && t * SK + k >= p.steps) break;
-            if (PHASED && k == 0) {
-                store(next, t + 1);
-                __builtin_amdgcn_sched_barrier(0);
-            }
-            v8i fa[RT], fb[CT];
-            int sa[(RT + 3) / 4], sb[(CT + 3) / 4];
+        for (int u = 0; u < RT; ++u) f.a[u] = a.fragment(image + buf * OpA::BYTES, u, k);
 #pragma unroll
-            for (int u = 0; u < RT; ++u) fa[u] = a.fragment(image + buf * OpA::BYTES, u, k);
+        for (int w = 0; w < CT; ++w) f.b[w] = b.fragment(image + B_AT + buf * OpB::BYTES, w, k);
 #pragma unroll
-            for (int w = 0; w < CT; ++w) fb[w] = b.fragment(image + B_AT + buf * OpB::BYTES, w, k);
+        for (int q = 0; q < (RT + 3) / 4; ++q) f.sa[q] = (int)(lscale[buf][k][wm * RT / 4 + q][lane] >> first_a);
 #pragma unroll
-            for (int q = 0; q < (RT + 3) / 4; ++q) sa[q] = *reinterpret_cast<const int *>(&lscale[buf][k][wm * RT / 4 + q][g][r][0]) >> first_a;
+        for (int q = 0; q < (CT + 3) / 4; ++q) f.sb[q] = (int)(lscale[buf][k][GA + wn * CT / 4 + q][lane] >> first_b);
+    };
+    const auto multiply = [&](const Fragments &f) {
 #pragma unroll
-            for (int q = 0; q < (CT + 3) / 4; ++q) sb[q] = *reinterpret_cast<const int *>(&lscale[buf][k][GA + wn * CT / 4 + q][g][r][0]) >> first_b;
-            if (PHASED) {
-                if (k == 0) load(next, t + 1 + AHEAD);
-                // the load path and the LDS work side by side: a load after every few fragment reads
-                constexpr int READS = RT * OpA::S1 / 64 + CT * OpB::S1 / 64 + RT / 4 + CT / 4, LOADS = OpA::MOVES + OpB::MOVES + SMOVES;
+        for (int w = 0; w < CT; ++w)
 #pragma unroll
-                for (int q = 0; q < LOADS; ++q) {
-                    __builtin_amdgcn_sched_group_barrier(0x100, READS / LOADS, 0);
-                    __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-                }
-                __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
-                __builtin_amdgcn_sched_barrier(0);
-                __syncthreads();
-                __builtin_amdgcn_s_setprio(1);
-            }
-#pragma unroll
-            for (int w = 0; w < CT; ++w)
-#pragma unroll
-                for (int u = 0; u < RT; ++u)
-                    acc[u][w] = mma_bytes<FA, FB>(fb[w], fa[u], acc[u][w], sb[w / 4], w, sa[u / 4], u);
-            if (PHASED) {
-                __builtin_amdgcn_s_setprio(0);
-                __builtin_amdgcn_sched_barrier(0);
-                __syncthreads();
-            }
-        }
-        if (!PHASED) {
-            store(next, t + 1);
-            load(next, t + 1 + AHEAD);
-            __syncthreads();
-        }
+            for (int u = 0; u < RT; ++u) acc[u][w] = mma_bytes<FA, FB>(f.b[w], f.a[u], acc[u][w], f.sb[w / 4], w, f.sa[u / 4], u);
     };
     Stage odd, even;                                         // (AHEAD 1: every stage goes through `odd`)
     load(odd, 0);
@@ -511,14 +492,51 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     store(odd, 0);
     load(odd, AHEAD);
     __syncthreads();
-    if (PHASED && wave >= 4) __syncthreads();
-    if (AHEAD == 1) {
-        for (int t = 0; t < stages; ++t) step(t, odd);
-    } else {
-        for (int t = 0; t < stages; t += 2) {
-            step(t, even);
-            if (t + 1 < stages) step(t + 1, odd);
+    if constexpr (PHASED) {
+        static_assert(SK == 1 && AHEAD == 1, "one depth a stage");
+        constexpr int READS = RT * OpA::S1 / 64 + CT * OpB::S1 / 64 + RT / 4 + CT / 4, LOADS = OpA::MOVES + OpB::MOVES + SMOVES;
+        if (wave >= 4) __syncthreads();
+        for (int t = 0; t < stages; ++t) {
+            store(odd, t + 1);
+            __builtin_amdgcn_sched_barrier(0);
+            Fragments f;
+            read(f, t, 0);
+            load(odd, t + 1 + AHEAD);
+            // the load path and the LDS work side by side: a load after every few fragment reads
+#pragma unroll
+            for (int q = 0; q < LOADS; ++q) {
+                __builtin_amdgcn_sched_group_barrier(0x100, READS / LOADS, 0);
+                __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            }
+            __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
+            __builtin_amdgcn_s_setprio(1);
+            multiply(f);
+            __builtin_amdgcn_s_setprio(0);
+            __builtin_amdgcn_sched_barrier(0);
+            __syncthreads();
         }
+    } else {
+        Fragments f[2];                                      // (the last read is of the stage behind the end; not multiplied)
+        read(f[0], 0, 0);
+        const auto step = [&](int t, Stage &next, int at) {  // `at`: which of f holds the stage's first depth
+#pragma unroll
+            for (int k = 0; k < SK; ++k) {
+                if (k == SK - 1) {
+                    store(next, t + 1);
+                    load(next, t + 1 + AHEAD);
+                    __syncthreads();
+                }
+                read(f[(at + k + 1) & 1], t + (k + 1) / SK, (k + 1) % SK);
+                multiply(f[(at + k) & 1]);
+            }
+        };
+        for (int t = 0; t + 1 < stages; t += 2) {
+            step(t, AHEAD == 1 ? odd : even, 0);
+            step(t + 1, odd, SK & 1);
+        }
+        if (stages & 1) step(stages - 1, AHEAD == 1 ? odd : even, 0);
     }
     if (PHASED && wave < 4) __syncthreads();
     uint8_t *room = image + wave * 2048;

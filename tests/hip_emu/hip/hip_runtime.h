@@ -266,6 +266,27 @@ template <class T> static inline T emu_buffer_load(__amdgpu_buffer_rsrc_t r, int
 #define __builtin_amdgcn_raw_buffer_load_b128(r, at, base, aux) emu_buffer_load<emu_u32x4>((r), (at) + (base))
 #define __builtin_amdgcn_raw_buffer_load_b32(r, at, base, aux) emu_buffer_load<unsigned>((r), (at) + (base))
 #define __builtin_amdgcn_make_buffer_rsrc(p, stride, size, flags) emu_make_rsrc((p), (size))
+// bytes of two words (0 .. 3: the second's, 4 .. 7: the first's); lanes 32 or 16 apart: [0] the pair's word with that lane bit clear, [1] set
+static inline unsigned emu_perm(unsigned hi, unsigned lo, unsigned sel) {
+    unsigned out = 0;
+    for (int k = 0; k < 4; ++k) {
+        const unsigned s = (sel >> (8 * k)) & 7;
+        out |= (((s < 4 ? lo : hi) >> (8 * (s & 3))) & 255u) << (8 * k);
+    }
+    return out;
+}
+struct emu_pair { unsigned w[2]; unsigned operator[](int k) const { return w[k]; } };
+static inline emu_pair emu_lane_pair(int site, unsigned w, int apart) {
+    const char *all = emu::gather(site, &w, 4);
+    const int lane = (int)(emu::tid_x() & 63);
+    emu_pair out;
+    memcpy(&out.w[0], all + (lane & ~apart) * emu::GATHER_MAX, 4);
+    memcpy(&out.w[1], all + (lane | apart) * emu::GATHER_MAX, 4);
+    return out;
+}
+#define __builtin_amdgcn_perm(hi, lo, sel) emu_perm((hi), (lo), (sel))
+#define __builtin_amdgcn_permlane32_swap(a, b, fi, bc) emu_lane_pair(__COUNTER__, (a), 32)
+#define __builtin_amdgcn_permlane16_swap(a, b, fi, bc) emu_lane_pair(__COUNTER__, (a), 16)
 // conversions of two codes back: value * 2^(exponent field of the scale - 127), rounded once to the output's type
 typedef float emu_f32x2 __attribute__((ext_vector_type(2)));
 static inline double emu_scaled(int fmt, unsigned code, float scale) {
