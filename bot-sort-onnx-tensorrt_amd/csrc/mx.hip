@@ -11,7 +11,8 @@ typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 
 // ---- quantisation and back: one thread per 8 elements, four lanes per block, 16 lanes per 128 padded elements ------------------
-// Groups of 16 lanes walk the 128-element pieces of all rows (their number fits 32 bits: the host's check).
+// Groups of 16 lanes walk the 128-element pieces of all rows (their number fits 32 bits: the host's check).  Memory bounds both ways:
+// 65536 x 2048 bfloat16 to E2M1, 340 MB, in 77 us (4.4 TB/s), back in 60 us (5.6 TB/s).
 template <class T, int FMT>
 __global__ __launch_bounds__(256) void k_mx_quantize(const T *__restrict__ x, long ldx, uint32_t pieces, uint32_t row_pieces, int d,
                                                      uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
@@ -116,7 +117,7 @@ template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const N
 
 // TPR threads per row, CH pieces of 8 elements a thread: the row stays in registers between the sum and the output, so x and residual
 // are read once.  CH = 0: rows beyond 8192 elements, in two passes; the second reads the stored sum, or x and residual again.
-// One pass over memory bounds it: 32768 x 4096 bfloat16 with residual and weight, 0.94 GB in 163 us (5.8 TB/s).
+// One pass over memory bounds it: 32768 x 4096 bfloat16 with residual and weight, 0.94 GB in 177 us (5.3 TB/s).
 template <class T, int TPR, int CH, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
     __shared__ double part[4];
@@ -246,8 +247,8 @@ template <class T> __device__ __forceinline__ void epilogue4(const ProductArgs &
 }
 
 // A workgroup of 4 wavefronts computes one 16 x 16 tile straight from memory; each wavefront takes a quarter of the row, and the parts are
-// added through LDS in a fixed order.  For few tiles, where the length of a row is what takes time (1 x 2000 x 2048: 3.6 us against 5.4
-// with LDS tiles; 1 x 300 x 8192: 7.4 against 12.4), and for sizes beyond the tiles' 32-bit offsets.
+// added through LDS in a fixed order.  For few tiles, where the length of a row is what takes time (1 x 2000 x 2048: 3.5 us against 5.2
+// with LDS tiles; 1 x 300 x 8192: 6.7 against 12.2), and for sizes beyond the tiles' 32-bit offsets.
 template <int FA, int FB>
 __global__ __launch_bounds__(256) void k_mx_direct(ProductArgs p) {
     __shared__ v4f part[3][64];
@@ -405,9 +406,10 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
 // other fetches its fragments, stores the next stage and issues the loads of the one after; barriers keep the two in step.  With 4
 // wavefronts a stage has one barrier, a depth's fragments are read while the one before it is multiplied (1000 x 1000 x 1000: 5.2 us
 // against 6.6 with both in turn), and the workgroups of a CU overlap.
-// What bounds it (128 x 128, E2M1 x E2M1, 10240 x 2048 x 8192, 128 us): the output and the instructions alone take 80, the writes to LDS 29
-// more, the loads behind them 25; fragment reads cost nothing.  A round of tiles computes and then stores together, so the output of
-// 10000 x 2000 float32 (17 us) comes on top of the loop (14 us per 1024 elements of depth).
+// What bounds it (128 x 128, E2M1 x E2M1, 10240 x 2048 x 8192, 130 us): the matrix instructions, the fragment reads and the output take 77,
+// the writes to LDS 25 more, the loads 28; the reads cost nothing beside the instructions.  A round of tiles computes and then stores together, so the output of
+// 10000 x 2000 float32 (17 us) comes on top of the loop (14 us per 1024 elements of depth).  256 x 256 tiles of E4M3 x E2M1, 16384 x 8192 x
+// 4096: 440 us, 2.5 PFLOP/s; the same with zeros in all codes is a quarter faster, that is the card's power limit.
 template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     constexpr int THREADS = 64 * WM * WN, RT = TM / WM / 16, CT = TN / WN / 16;
@@ -613,12 +615,14 @@ template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> voi
             [&](dim3 grid) { hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK, AHEAD>), grid, dim3(64 * WM * WN), 0, st, p); });
 }
 // Which kernel: by how many workgroups the sizes make of the chip, measured at d = 2048 unless said otherwise (us, E4M3 x E2M1).
-//  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 439 against
-//    630; 10000 x 2000, 320 tiles in two rounds: 61 against 55).  Two E4M3 operands' images of 256 rows do not fit.
-//  - 128 x 128 tiles from two a CU on (10000 x 2000: 56 against 75 with 64 x 64 ones; 2000 x 2000 x 1000, one a CU: 14.7 against 12.0).
-//  - 64 x 64 tiles from one a CU on (48 x 65536: 19; 1000 x 1000 x 1000: 6.6 against 11), below that 16 x 64 ones (200 x 2000 x 1024: 4.9 against
-//    6.0), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.5 against 18).
-//  - 16 x 16 tiles with the row split where there are fewer than two of them a CU (1 x 2000: 3.6 against 5.4).
+//  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 408 against
+//    613; 6000 x 2000, one round: 28 against 35; 10000 x 2000, 320 tiles in two rounds: 53 against 55, with E2M1 on both sides 55 against
+//    43).  Two E4M3 operands' images of 256 rows do not fit.
+//  - 128 x 128 tiles from two a CU on (2000 x 2000 x 1024, one a CU: 12.2 against 11.7 with 64 x 64 ones).
+//  - 64 x 64 tiles from one a CU on (48 x 65536: 20; 1000 x 1000 x 1000: 5.9), below that 16 x 64 ones (for these two 27 and 6.6; 200 x 2000 x
+//    1024: 4.8 against 5.3), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.7 against 18).
+//  - 16 x 16 tiles with the row split where there are fewer of them than CUs (1 x 2000: 3.5 against 5.2; 16 x 3000 x 512: 2.9 against 3.6;
+//    300 x 300 x 1000, one and a half a CU: 4.6 against 4.1).
 template <int FA, int FB> int product(bts_context *ctx, ProductArgs p, hipStream_t st) {
     const auto tiles = [&](long a, long b) { return ((p.n + a - 1) / a) * ((p.m + b - 1) / b); };
     const long cus = ctx->n_cu, t256 = tiles(256, 256), t128 = tiles(128, 128), most = 1L << 31;
@@ -627,7 +631,7 @@ template <int FA, int FB> int product(bts_context *ctx, ProductArgs p, hipStream
     constexpr bool BIG = FA == E2M1 || FB == E2M1;
     // 32-bit offsets inside a tile: 256 rows of codes, 16 rows of the output
     const bool fits = (long)p.steps * 128 * 256 < most && p.ld * 4 * 16 < most && p.n < most - 256 && p.m < most - 256;
-    if (!fits || tiles(16, 16) < 2 * cus) {
+    if (!fits || tiles(16, 16) < cus) {
         in_runs(p, tiles(16, 16), [&](dim3 grid) { hipLaunchKernelGGL((k_mx_direct<FA, FB>), grid, dim3(256), 0, st, p); });
         BTS_LAUNCH_CHECK();
         return BTS_OK;
