@@ -57,6 +57,8 @@ def _rows2d(t, name, like=None):
         raise _lib.BtsError("%s: a device tensor is expected" % name)
     if t.dim() != 2:
         raise _lib.BtsError("%s: [rows, d] expected, got %d dimensions" % (name, t.dim()))
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _lib.BtsError("%s: no gradient is formed here: detach it or call under torch.no_grad()" % name)
     n, d = t.shape
     ld, unit = t.stride()
     if n <= 1:
@@ -90,7 +92,9 @@ class MxRows:
     """n rows of d values in microscaled form: `codes` uint8 [n, code bytes], `scales` uint8 [n, d rounded up to 128, / 32], `fmt`
     "e2m1" (two elements a byte, the even one in the low nibble) or "e4m3".  Element = code value * 2^(scale - 127); scale 255 = NaN.
     The layout is include/botsort_hip.h's: a consumer may fill the tensors itself."""
-    __slots__ = ("codes", "scales", "d", "fmt", "_code")
+    # rows made here lie in one allocation, codes before scales; the two tensors are views made when asked for (an allocation and two views
+    # less: 2 us of an 8 us call)
+    __slots__ = ("d", "fmt", "device", "_code", "_n", "_room", "_codes", "_scales")
 
     def __init__(self, codes, scales, d: int, fmt: str):
         if torch is None:
@@ -106,20 +110,38 @@ class MxRows:
             raise _lib.BtsError("MxRows: codes and scales on one GPU expected")
         if not (codes.is_contiguous() and scales.is_contiguous()):
             raise _lib.BtsError("MxRows: contiguous codes and scales expected")
-        self.codes, self.scales, self.d, self.fmt = codes, scales, d, fmt
+        self.d, self.fmt, self.device, self._n, self._room, self._codes, self._scales = d, fmt, codes.device, n, None, codes, scales
 
-    @classmethod
-    def _of(cls, codes, scales, d, fmt, code):
-        """Rows of tensors that this module has made itself."""
-        self = cls.__new__(cls)
-        self.codes, self.scales, self.d, self.fmt, self._code = codes, scales, d, fmt, code
-        return self
+    def _pointers(self):
+        if self._room is None:
+            return self._codes.data_ptr(), self._scales.data_ptr()
+        at = self._room.data_ptr()
+        return at, at + self._n * self._widths()[0]
+
+    def _widths(self):
+        """(code bytes, scale bytes) of a row"""
+        wide = (self.d + _ROW - 1) // _ROW * _ROW
+        return wide // 2 if self._code == 0 else wide, wide // _BLOCK
+
+    @property
+    def codes(self):
+        if self._codes is None:
+            c, n = self._widths()[0], self._n
+            self._codes = self._room[:n * c].view(n, c)
+        return self._codes
+
+    @property
+    def scales(self):
+        if self._scales is None:
+            (c, t), n = self._widths(), self._n
+            self._scales = self._room[n * c:].view(n, t)
+        return self._scales
 
     def __len__(self):
-        return self.codes.shape[0]
+        return self._n
 
     def __repr__(self):
-        return "MxRows(%d x %d, %s, %s)" % (len(self), self.d, self.fmt, self.codes.device)
+        return "MxRows(%d x %d, %s, %s)" % (self._n, self.d, self.fmt, self.device)
 
     @classmethod
     def empty(cls, n: int, d: int, fmt: str, device="cuda") -> "MxRows":
@@ -129,9 +151,11 @@ class MxRows:
         code, wide = _format_code(fmt), _width(d)
         if not 0 <= n <= _MOST:
             raise _lib.BtsError("MxRows: 0 .. 2^31 - 1 rows, got %d" % n)
-        device = torch.device(device)
-        return cls._of(torch.empty((n, wide // 2 if code == 0 else wide), dtype=torch.uint8, device=device),
-                       torch.empty((n, wide // _BLOCK), dtype=torch.uint8, device=device), int(d), fmt, code)
+        self = cls.__new__(cls)
+        self.d, self.fmt, self._code, self._n, self._codes, self._scales = int(d), fmt, code, n, None, None
+        self._room = torch.empty(n * ((wide // 2 if code == 0 else wide) + wide // _BLOCK), dtype=torch.uint8, device=device)
+        self.device = self._room.device
+        return self
 
     def dequantize(self, dtype=None):
         """[n, d] of the values held (float32 unless `dtype` says otherwise)."""
@@ -139,29 +163,31 @@ class MxRows:
             _init()
         dtype = torch.float32 if dtype is None else dtype
         code = _dtype_code(dtype)
-        n, d = self.codes.shape[0], self.d
-        out = torch.empty((n, d), dtype=dtype, device=self.codes.device)
-        lib, ctx, stream = _call(self.codes.device)
-        _lib.check(lib.bts_mx_dequantize(ctx, self.codes.data_ptr(), self.scales.data_ptr(), self._code, n, d, out.data_ptr(), code, d, stream))
+        n, d = self._n, self.d
+        out = torch.empty((n, d), dtype=dtype, device=self.device)
+        lib, ctx, stream = _call(self.device)
+        pc, ps = self._pointers()
+        _lib.check(lib.bts_mx_dequantize(ctx, pc, ps, self._code, n, d, out.data_ptr(), code, d, stream))
         return out
 
 
 def _room(out, n, d, fmt, device):
     if out is None:
         return MxRows.empty(n, d, fmt, device)
-    if len(out) != n or out.d != d or out.fmt != fmt or out.codes.device != device:
+    if out._n != n or out.d != d or out.fmt != fmt or out.device != device:
         raise _lib.BtsError("out: %d x %d rows in %s on %s expected, got %r" % (n, d, fmt, device, out))
     return out
 
 
 def mx_quantize(x, fmt: str = "e2m1", out: MxRows = None) -> MxRows:
     """x [n, d] (float32, float16 or bfloat16; rows may be strided) -> its rows in 4 (e2m1) or 8 (e4m3) bits; `out`: rows to fill."""
-    p, ld = _rows2d(x, "x")
     dt, f = _dtype_code(x.dtype), _format_code(fmt)
+    p, ld = _rows2d(x, "x")
     n, d = x.shape
     out = _room(out, n, d, fmt, x.device)
     lib, ctx, stream = _call(x.device)
-    _lib.check(lib.bts_mx_quantize(ctx, p, dt, ld, n, d, f, out.codes.data_ptr(), out.scales.data_ptr(), stream))
+    pc, ps = out._pointers()
+    _lib.check(lib.bts_mx_quantize(ctx, p, dt, ld, n, d, f, pc, ps, stream))
     return out
 
 
@@ -170,12 +196,14 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     -> (rows in `fmt`, h).  fmt=None: no quantised rows, only `y_out`.
 
     `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` the normalised rows in x's type."""
-    px, ldx = _rows2d(x, "x")
     dt = _dtype_code(x.dtype)
+    px, ldx = _rows2d(x, "x")
     n, d = x.shape
     pr, ldr = _rows2d(residual, "residual", x) if residual is not None else (None, 0)
     if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous()):
         raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
+    if weight is not None and weight.requires_grad and torch.is_grad_enabled():
+        raise _lib.BtsError("weight: no gradient is formed here: detach it or call under torch.no_grad()")
     if sum_out is None and residual is not None:
         sum_out = torch.empty((n, d), dtype=x.dtype, device=x.device)
     ps, lds = _rows2d(sum_out, "sum_out", x) if sum_out is not None else (None, 0)
@@ -185,8 +213,9 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     f = 0 if fmt is None else _format_code(fmt)
     rows = None if fmt is None else _room(out, n, d, fmt, x.device)
     lib, ctx, stream = _call(x.device)
+    qc, qs = (None, None) if rows is None else rows._pointers()
     _lib.check(lib.bts_rms_norm(ctx, dt, px, ldx, pr, ldr, None if weight is None else weight.data_ptr(), n, d, float(eps), ps, lds, py, ldy, f,
-                                None if rows is None else rows.codes.data_ptr(), None if rows is None else rows.scales.data_ptr(), stream))
+                                qc, qs, stream))
     return rows, x if sum_out is None else sum_out
 
 
@@ -197,10 +226,10 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
     `out`: a matrix to fill (its type counts; rows may be strided)."""
     if not isinstance(a, MxRows) or not isinstance(b, MxRows):
         raise _lib.BtsError("mx_product: MxRows expected")
-    device = a.codes.device
-    if a.d != b.d or b.codes.device != device:
+    device = a.device
+    if a.d != b.d or b.device != device:
         raise _lib.BtsError("mx_product: rows of one width on one device expected, got %r and %r" % (a, b))
-    n, m = a.codes.shape[0], b.codes.shape[0]
+    n, m = a._n, b._n
     if out is None:
         if dtype is None:
             dtype = torch.float32 if a.fmt == b.fmt == "e2m1" else torch.bfloat16
@@ -212,6 +241,6 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
             raise _lib.BtsError("out: [%d, %d] on %s%s expected" % (n, m, device, "" if dtype is None else " of %s" % dtype))
     po, ld = _rows2d(out, "out")
     lib, ctx, stream = _call(device)
-    _lib.check(lib.bts_mx_product(ctx, a.codes.data_ptr(), a.scales.data_ptr(), a._code, n, b.codes.data_ptr(), b.scales.data_ptr(), b._code,
-                                  m, a.d, float(alpha), 1 if floor_zero else 0, po, code, ld, stream))
+    (ac, as_), (bc, bs) = a._pointers(), b._pointers()
+    _lib.check(lib.bts_mx_product(ctx, ac, as_, a._code, n, bc, bs, b._code, m, a.d, float(alpha), 1 if floor_zero else 0, po, code, ld, stream))
     return out

@@ -487,6 +487,31 @@ def test_gallery_search_as_it_is_used(bts, gallery, queries, d, fa, fmt):
     assert np.abs(sim - full).max() <= 2 * 6 * 0.12 / math.sqrt(d) + 2 ** -8
 
 
+def test_a_slice_of_rows(bts):
+    """rows built from parts of other rows' tensors, written in place as well"""
+    x = torch.from_numpy(feature_rows(9, 200, 4)).float().cuda()
+    for fmt in ("e2m1", "e4m3"):
+        q = bts.mx_quantize(x, fmt)
+        part = bts.MxRows(q.codes[3:7], q.scales[3:7], 200, fmt)
+        assert len(part) == 4 and torch.equal(part.dequantize().cpu(), q.dequantize()[3:7].cpu())
+        assert q.codes.shape == (9, bts.mx_row_bytes(fmt, 200)[0]) and q.scales.shape == (9, bts.mx_row_bytes(fmt, 200)[1])
+        before = q.dequantize().cpu()
+        bts.mx_quantize(2 * x[3:7], fmt, out=part)                                  # (twice the values: the same codes, scales one up)
+        after = q.dequantize().cpu()
+        assert torch.equal(after[3:7], 2 * before[3:7]) and torch.equal(after[:3], before[:3]) and torch.equal(after[7:], before[7:])
+        assert torch.equal(bts.mx_product(part, q, dtype=torch.bfloat16).cpu(), bts.mx_product(q, q, dtype=torch.bfloat16).cpu()[3:7])
+
+
+def test_leaves_that_want_a_gradient(bts):
+    x, w = torch.ones((2, 64)).cuda().requires_grad_(), torch.ones(64).cuda().requires_grad_()
+    for call in (lambda: bts.mx_quantize(x), lambda: bts.rms_norm_mx(x), lambda: bts.rms_norm_mx(x.detach(), weight=w),
+                 lambda: bts.rms_norm_mx(x.detach(), residual=x)):
+        with pytest.raises(bts.BtsError):
+            call()
+    with torch.no_grad():
+        assert len(bts.mx_quantize(x)) == 2 and len(bts.rms_norm_mx(x, weight=w)[0]) == 2
+
+
 def test_two_runs_give_the_same_bits(bts):
     a, _ = rows_of(bts, feature_rows(150, 900, 7), "e4m3")
     b, _ = rows_of(bts, feature_rows(90, 900, 8), "e2m1")
