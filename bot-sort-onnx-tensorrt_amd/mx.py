@@ -195,7 +195,8 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     """Root-mean-square norm of the rows of h = x + residual (rounded to x's type; h = x without a residual), times `weight` [d]
     -> (rows in `fmt`, h).  fmt=None: no quantised rows, only `y_out`.
 
-    `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` the normalised rows in x's type."""
+    `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` (likewise) the normalised rows in x's type.
+    Without a residual h is x itself, or a copy where y_out takes its place."""
     dt = _dtype_code(x.dtype)
     px, ldx = _rows2d(x, "x")
     n, d = x.shape
@@ -204,10 +205,10 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
         raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
     if weight is not None and weight.requires_grad and torch.is_grad_enabled():
         raise _lib.BtsError("weight: no gradient is formed here: detach it or call under torch.no_grad()")
-    if sum_out is None and residual is not None:
+    py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
+    if sum_out is None and (residual is not None or py == px):      # (y in the place of x: h is x as it was)
         sum_out = torch.empty((n, d), dtype=x.dtype, device=x.device)
     ps, lds = _rows2d(sum_out, "sum_out", x) if sum_out is not None else (None, 0)
-    py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
     if fmt is None and out is not None:
         raise _lib.BtsError("out: rows to fill need their fmt")
     f = 0 if fmt is None else _format_code(fmt)

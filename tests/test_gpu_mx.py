@@ -262,6 +262,21 @@ def test_rms_norm_in_place(bts, d):
     assert torch.equal(xd.cpu(), y0.cpu())
 
 
+@pytest.mark.parametrize("d", [96, 1500, 9000])
+@pytest.mark.parametrize("fmt", ["e4m3", None])
+def test_rms_norm_in_the_place_of_x_returns_the_rows_that_were_there(bts, d, fmt):
+    """y in the place of x, no residual and no room for h: h is x as it was, not what was written over it"""
+    x = awkward(6, d, "bf16", d)
+    y0 = torch.empty_like(x).cuda()
+    q0, _ = bts.rms_norm_mx(x.cuda(), fmt=fmt, y_out=y0)
+    xd = x.cuda()
+    q, h = bts.rms_norm_mx(xd, fmt=fmt, y_out=xd)
+    assert torch.equal(h.cpu(), x) and torch.equal(xd.cpu().view(torch.int16), y0.cpu().view(torch.int16))
+    assert fmt is None or (torch.equal(q.codes.cpu(), q0.codes.cpu()) and torch.equal(q.scales.cpu(), q0.scales.cpu()))
+    xd, h1 = x.cuda(), torch.empty_like(x).cuda()
+    assert bts.rms_norm_mx(xd, fmt=fmt, y_out=xd, sum_out=h1)[1] is h1 and torch.equal(h1.cpu(), x)
+
+
 @pytest.mark.parametrize("d", [40, 1500, 9000])
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 def test_rms_norm_at_the_ends_of_the_range(bts, d, dtype):
