@@ -2,6 +2,8 @@
 // (with the residual's addition) that writes such rows, and their product on the matrix cores.  mx_math.h holds the format.
 #include "mx_math.h"
 
+#include <algorithm>
+
 namespace {
 
 using namespace mx;
@@ -562,6 +564,34 @@ dim3 piece_grid(const bts_context *ctx, long pieces) {
     return dim3((unsigned)(blocks < most ? blocks : most));
 }
 
+// Rows of `bytes` bytes, `stride` bytes apart (null: none).  Whether two sets of them share a byte -- the kernels read and write rows in no
+// order, so an output may not lie across an input; rows between another's rows are fine.
+struct Rows {
+    const void *p;
+    long n, bytes, stride;
+    bool same(const Rows &o) const { return p == o.p && stride == o.stride; }
+};
+Rows matrix(const void *p, long n, long d, long ld, int dtype) { return {p, n, d * (long)dtype_bytes(dtype), ld * (long)dtype_bytes(dtype)}; }
+Rows block(const void *p, long bytes) { return {p, 1, bytes, bytes}; }
+bool overlap(Rows a, Rows b) {
+    if (!a.p || !b.p) return false;
+    for (Rows *r : {&a, &b})
+        if (r->n == 1 || r->bytes == r->stride) *r = block(r->p, r->n * r->bytes);
+    const long at = (intptr_t)a.p, to = (intptr_t)b.p;
+    if (at + (a.n - 1) * a.stride + a.bytes <= to || to + (b.n - 1) * b.stride + b.bytes <= at) return false;
+    const auto floor_div = [](long v, long by) { return v / by - (v % by < 0); };
+    if (a.n > 1 && a.stride == b.stride) {         // the first row distance at which b's row does not end before a's begins
+        const long k = std::max(floor_div(at - to - b.bytes, a.stride) + 1, 1 - a.n);
+        return k < b.n && to + k * a.stride < at + a.bytes;
+    }
+    if (a.n > b.n) return overlap(b, a);
+    for (long i = 0; i < a.n; ++i) {
+        const long from = at + i * a.stride, j = std::max(floor_div(from - to - b.bytes, b.stride) + 1, 0l);
+        if (j < b.n && to + j * b.stride < from + a.bytes) return true;
+    }
+    return false;
+}
+
 template <class T> void quantize(bts_context *ctx, const void *x, int ldx, int n, int d, int format, uint8_t *codes, uint8_t *scales, hipStream_t st) {
     const uint32_t all = (uint32_t)pieces(n, d), row = (uint32_t)(padded(d) / MX_ROW);
     const T *const xs = static_cast<const T *>(x);
@@ -674,6 +704,8 @@ int bts_mx_quantize(bts_context *ctx, const void *x, int x_dtype, int ldx, int n
     BTS_REQUIRE(aligned(x, dtype_bytes(x_dtype)) && aligned(codes, 16) && aligned(scales, 4), "x: element, codes: 16-byte, scales: 4-byte alignment");
     hipStream_t st = (hipStream_t)stream;
     BTS_REQUIRE(pieces(n, d) <= MOST_PIECES, "n * d: too many elements for one call");
+    const Rows xs = matrix(x, n, d, ldx, x_dtype), cs = block(codes, n * mx::code_bytes(format, d)), ss = block(scales, n * mx::scale_bytes(d));
+    BTS_REQUIRE(!overlap(cs, ss) && !overlap(xs, cs) && !overlap(xs, ss), "x, codes and scales overlap");
     if (x_dtype == BTS_F32) quantize<float>(ctx, x, ldx, n, d, format, codes, scales, st);
     else if (x_dtype == BTS_F16) quantize<_Float16>(ctx, x, ldx, n, d, format, codes, scales, st);
     else quantize<bf16>(ctx, x, ldx, n, d, format, codes, scales, st);
@@ -691,6 +723,9 @@ int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *sca
     BTS_REQUIRE(aligned(out, dtype_bytes(out_dtype)) && aligned(codes, 16) && aligned(scales, 4), "out: element, codes: 16-byte, scales: 4-byte alignment");
     hipStream_t st = (hipStream_t)stream;
     BTS_REQUIRE(pieces(n, d) <= MOST_PIECES, "n * d: too many elements for one call");
+    const Rows os = matrix(out, n, d, ldo, out_dtype);
+    BTS_REQUIRE(!overlap(os, block(codes, n * mx::code_bytes(format, d))) && !overlap(os, block(scales, n * mx::scale_bytes(d))),
+                "out overlaps codes or scales");
     if (out_dtype == BTS_F32) dequantize<float>(ctx, codes, scales, format, n, d, out, ldo, st);
     else if (out_dtype == BTS_F16) dequantize<_Float16>(ctx, codes, scales, format, n, d, out, ldo, st);
     else dequantize<bf16>(ctx, codes, scales, format, n, d, out, ldo, st);
@@ -706,10 +741,6 @@ int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void
     BTS_REQUIRE(!residual || ldr >= d, "ldr < d");
     BTS_REQUIRE(!sum || lds >= d, "lds < d");
     BTS_REQUIRE(!y || ldy >= d, "ldy < d");
-    BTS_REQUIRE(!y || (y != sum && y != weight), "y may not be sum or weight");
-    BTS_REQUIRE(!sum || sum != weight, "sum may not be weight");
-    BTS_REQUIRE(!sum || ((sum != x || lds == ldx) && (sum != residual || lds == ldr)), "sum in the place of x / residual needs their row stride");
-    BTS_REQUIRE(!y || ((y != x || ldy == ldx) && (y != residual || ldy == ldr)), "y in the place of x / residual needs their row stride");
     BTS_ON_DEVICE(ctx);
     if (n == 0) return BTS_OK;
     BTS_REQUIRE(x, "null pointer");
@@ -719,6 +750,15 @@ int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void
     const size_t b = dtype_bytes(dtype);
     BTS_REQUIRE(aligned(x, b) && aligned(residual, b) && aligned(weight, b) && aligned(sum, b) && aligned(y, b), "element alignment");
     BTS_REQUIRE(aligned(codes, 16) && aligned(scales, 4), "codes: 16-byte, scales: 4-byte alignment");
+    const Rows xs = matrix(x, n, d, ldx, dtype), rs = matrix(residual, n, d, ldr, dtype), ws = matrix(weight, 1, d, d, dtype);
+    const Rows hs = matrix(sum, n, d, lds, dtype), ys = matrix(y, n, d, ldy, dtype);
+    const Rows cs = block(codes, codes ? n * mx::code_bytes(format, d) : 0), ss = block(scales, n * mx::scale_bytes(d));
+    for (const Rows &to : {hs, ys})
+        BTS_REQUIRE((to.same(xs) || !overlap(to, xs)) && (to.same(rs) || !overlap(to, rs)) && !overlap(to, ws),
+                    "sum and y may take the place of x or residual (with its row stride), and may not overlap them or weight otherwise");
+    BTS_REQUIRE(!overlap(hs, ys) && !overlap(cs, ss), "sum and y, or codes and scales, overlap");
+    for (const Rows &to : {cs, ss})
+        for (const Rows &of : {xs, rs, ws, hs, ys}) BTS_REQUIRE(!overlap(to, of), "codes or scales overlap a matrix");
     hipStream_t st = (hipStream_t)stream;
     const int f = codes ? format : -1;
     if (dtype == BTS_F32) rms_norm<float>(x, ldx, residual, ldr, weight, n, d, eps, sum, lds, y, ldy, f, codes, scales, st);
@@ -740,6 +780,10 @@ int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_sc
     BTS_REQUIRE(a_codes && a_scales && b_codes && b_scales && out, "null pointer");
     BTS_REQUIRE(aligned(a_codes, 16) && aligned(b_codes, 16) && aligned(a_scales, 4) && aligned(b_scales, 4) && aligned(out, dtype_bytes(out_dtype)),
                 "codes: 16-byte, scales: 4-byte, out: element alignment");
+    const Rows os = matrix(out, n, m, ld, out_dtype);
+    for (const Rows &of : {block(a_codes, n * mx::code_bytes(a_format, d)), block(a_scales, n * mx::scale_bytes(d)),
+                           block(b_codes, m * mx::code_bytes(b_format, d)), block(b_scales, m * mx::scale_bytes(d))})
+        BTS_REQUIRE(!overlap(os, of), "out overlaps an operand");
     const size_t b = dtype_bytes(out_dtype);
     ProductArgs p;
     p.a_codes = a_codes; p.a_scales = a_scales; p.b_codes = b_codes; p.b_scales = b_scales;

@@ -169,7 +169,8 @@ int bts_feature_renorm(bts_context *ctx, float *feats, const int32_t *idx, int k
  * zero-padded to a multiple of 128 elements; rows follow each other without gaps.  codes: 16-byte, scales: 4-byte aligned.
  * Quantisation (OCP microscaling formats): s = 127 + clamp(floor(log2(max |v|)) - emax, -127, 127), emax = 2 (E2M1) / 8 (E4M3),
  * elements v / 2^(s - 127) rounded to nearest even, saturating.  A block with an infinity or a NaN in it becomes NaN.
- * Types of x / out / y: BTS_F32, BTS_F16 or BTS_BF16 (enum bts_dtype); row strides (ld*) are in elements, >= d; d <= 2^30. */
+ * Types of x / out / y: BTS_F32, BTS_F16 or BTS_BF16 (enum bts_dtype); row strides (ld*) are in elements, >= d; d <= 2^30.
+ * Outputs may not share memory with inputs or with each other, except where a call says so; rows between another's rows are fine. */
 enum bts_mx_format { BTS_MX_E2M1 = 0, BTS_MX_E4M3 = 1 };
 
 /* Bytes of one row's codes and scales (host-only). */

@@ -607,6 +607,75 @@ def test_c_entry_refusals(bts):
     assert (x.cpu() == 1).all() and (o.cpu() == 0).all()
 
 
+def shares(a, b):
+    """whether two sets of rows (place, rows, bytes a row, bytes between rows) share a byte, byte by byte"""
+    put = lambda r: {r[0] + i * r[3] + k for i in range(r[1]) for k in range(r[2])}  # noqa: E731
+    return bool(put(a) & put(b))
+
+
+def test_outputs_that_share_memory_are_refused(bts):
+    """every place of one output against one input inside a small buffer, decided by the bytes they share: y and x of the norm, of equal and of
+    different row strides; refused before anything is launched, and accepted when they only lie between each other's rows"""
+    lib, ctx = bts._lib.load(), bts._lib.default_context().handle
+    buf = torch.ones(600).cuda()
+    seen = set()
+    for n, d, ldx, ldy in ((3, 4, 12, 12), (3, 4, 9, 9), (4, 3, 7, 11), (1, 5, 5, 5), (5, 4, 4, 4), (4, 2, 13, 5)):
+        at = 150
+        for to in range(at - n * max(ldx, ldy) - d - 1, at + n * max(ldx, ldy) + d + 2):
+            want = shares((4 * at, n, 4 * d, 4 * ldx), (4 * to, n, 4 * d, 4 * ldy)) and not (to == at and ldx == ldy)
+            before = buf.cpu()
+            rc = lib.bts_rms_norm(ctx, 1, buf.data_ptr() + 4 * at, ldx, None, 0, None, n, d, 1e-6, None, 0, buf.data_ptr() + 4 * to, ldy, 0, None, None, None)
+            assert rc == (-1 if want else 0), (n, d, ldx, ldy, to - at)
+            if want:
+                assert torch.equal(buf.cpu(), before)
+            buf.fill_(1.0)
+            seen.add((want, ldx == ldy))
+    assert len(seen) == 4
+
+
+def test_overlapping_tensors_are_refused(bts):
+    x = torch.ones((6, 400)).cuda()
+    a, b, w = x[:, :128], x[:, 8:136], torch.ones(128).cuda()
+    raw = torch.zeros(40000, dtype=torch.uint8).cuda()
+    rows = lambda at, n, fmt="e4m3": bts.MxRows(raw[at:at + n * bts.mx_row_bytes(fmt, 128)[0]].view(n, -1),  # noqa: E731
+                                                raw[at + 20000:at + 20000 + 4 * n].view(n, 4), 128, fmt)
+    q = bts.mx_quantize(a, "e4m3", out=rows(0, 6))
+    f32 = lambda at, n, d: raw[at:at + 4 * n * d].view(torch.float32).view(n, d)  # noqa: E731
+    bad = [
+        lambda: bts.rms_norm_mx(a, sum_out=b),
+        lambda: bts.rms_norm_mx(a, y_out=b),
+        lambda: bts.rms_norm_mx(x[:5, :128], y_out=x[1:, :128]),                       # the same columns, a row further
+        lambda: bts.rms_norm_mx(a, residual=x[:, 200:328], sum_out=x[:, 201:329]),
+        lambda: bts.rms_norm_mx(a, residual=x[:, 200:328], sum_out=a, y_out=x[:, 127:255]),
+        lambda: bts.rms_norm_mx(a, residual=b, sum_out=a),                             # in the place of x, across residual
+        lambda: bts.rms_norm_mx(a, sum_out=x[:, 200:328], y_out=x[:, 272:]),
+        lambda: bts.rms_norm_mx(a, weight=x[3, :128], sum_out=a),                      # the weight is a row of what is written
+        lambda: bts.rms_norm_mx(a, weight=x[2, 272:], y_out=x[:, 272:]),
+        lambda: bts.rms_norm_mx(f32(0, 2, 128), out=rows(512, 2)),                     # codes over x
+        lambda: bts.rms_norm_mx(f32(20400, 2, 128), out=rows(512, 2)),                 # scales over x
+        lambda: bts.rms_norm_mx(a[:4], y_out=f32(512, 4, 128), out=rows(256, 4)),
+        lambda: bts.mx_quantize(f32(256, 4, 128), "e4m3", out=rows(0, 4)),
+        lambda: bts.mx_quantize(f32(20008, 4, 128), "e4m3", out=rows(0, 4)),
+        lambda: bts.mx_product(rows(0, 4), rows(1024, 4), out=raw[1024:1024 + 32].view(torch.bfloat16).view(4, 4)),
+        lambda: bts.mx_product(rows(0, 4), rows(1024, 4), out=raw[20000:20032].view(torch.bfloat16).view(4, 4)),
+    ]
+    lib, ctx = bts._lib.load(), bts._lib.default_context().handle
+    before = x.cpu(), raw.cpu()
+    for k, f in enumerate(bad):
+        with pytest.raises(bts.BtsError):
+            f()
+            print("accepted", k)
+    assert lib.bts_mx_dequantize(ctx, raw.data_ptr(), raw.data_ptr() + 20000, 1, 6, 128, raw.data_ptr() + 512, 1, 128, None) == -1
+    assert lib.bts_mx_dequantize(ctx, raw.data_ptr(), raw.data_ptr() + 20000, 1, 6, 128, raw.data_ptr() + 20008, 1, 128, None) == -1
+    assert lib.bts_mx_quantize(ctx, x.data_ptr(), 1, 400, 6, 128, 1, raw.data_ptr(), raw.data_ptr() + 764, None) == -1      # scales in the codes
+    assert torch.equal(x.cpu(), before[0]) and torch.equal(raw.cpu(), before[1])
+    # columns of one matrix beside each other, a and b the same rows, the addition in place
+    h = bts.rms_norm_mx(a, residual=x[:, 128:256], sum_out=x[:, 256:384])[1]
+    assert (h == 2).all() and (x[:, :256] == 1).all()
+    assert bts.rms_norm_mx(a, residual=a, sum_out=a, weight=w)[1] is a and (a == 2).all()
+    assert bts.mx_product(q, q).shape == (6, 6)
+
+
 # ------------------------------------------------------------------------------------------- streams, graphs, threads (hardware)
 
 @pytest.mark.skipif("libbotsort_emu" in __import__("os").environ.get("BTS_LIB_PATH", ""), reason="needs real streams and graphs")
