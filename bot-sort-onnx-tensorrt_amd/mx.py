@@ -155,6 +155,8 @@ class MxRows:
         self.d, self.fmt, self._code, self._n, self._codes, self._scales = int(d), fmt, code, n, None, None
         self._room = torch.empty(n * ((wide // 2 if code == 0 else wide) + wide // _BLOCK), dtype=torch.uint8, device=device)
         self.device = self._room.device
+        if not self._room.is_cuda:
+            raise _lib.BtsError("MxRows: rows live on a GPU, got %s" % self.device)
         return self
 
     def dequantize(self, dtype=None):
