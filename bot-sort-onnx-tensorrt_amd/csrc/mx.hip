@@ -84,29 +84,37 @@ __device__ __forceinline__ double squares(const float (&h)[8]) {
     for (int e = 0; e < 8; ++e) t += (double)h[e] * (double)h[e];
     return t;
 }
-// A row's factor.  Where the row's norm passes 2^63 or stays below 2^-50, its elements are first scaled by 2^-64 or 2^64 and the factor by
-// the inverse, so that neither the factor nor the elements times the weight leave float32's range.
-struct Factor { float inv, first; };
-__device__ __forceinline__ Factor row_factor(double ss, int d, double eps) {
-    const float first = ss > 0x1p126 ? 0x1p-64f : ss < 0x1p-100 ? 0x1p64f : 1.0f;
-    return {(float)(1.0 / (sqrt(ss / (double)d + eps) * (double)first)), first};
+// A row's factor as m * 2^e, m in [1, 2).  With a weight the elements are taken times 2^e first, so that their product with the weight is the
+// result but for m: it leaves float32's range only where the result does, however far the row's norm and the weight lie from 1 (a row
+// of 2^50 under a weight of 2^100).  Powers of two are exact, and for 16-bit types so is the product: one rounding follows that of the
+// factor.  The multiplication hides behind memory: 32768 x 4096 bfloat16 with residual and weight 164 us with and without it, 32768 x
+// 1111 float32 47.  Without a weight 2^e is apart only where the factor is subnormal.
+struct Factor { float m, power; };
+__device__ __forceinline__ Factor row_factor(double ss, int d, double eps, bool weight) {
+    const double full = 1.0 / sqrt(ss / (double)d + eps);
+    const float inv = (float)full;
+    if (!weight && inv >= 0x1p-126f) return {inv, 1.0f};
+    if (!(full >= 0x1p-130)) return {inv, inv};        // (a row with an infinity, 0, or a NaN)
+    int e;
+    const float m = (float)(2.0 * frexp(full, &e));    // (2 if it rounds up to that)
+    return {m, ldexpf(1.0f, e - 1)};
 }
 // the normalised piece at column k: to y, and as codes (whole blocks: a block's four lanes come together)
 template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const NormArgs<T> &a, long i, int k, int width, Factor f, float (&h)[8]) {
     if (k < a.d) {
         const int have = WHOLE ? 8 : a.d - k;
-        if (f.first != 1.0f) {
+        if (f.power != 1.0f) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] *= f.first;
+            for (int e = 0; e < 8; ++e) h[e] *= f.power;
         }
         if (a.weight) {
             float w[8];
             load8(a.weight + k, have, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) h[e] *= w[e];             // (exact for 16-bit types: one rounding, that of the factor, follows)
+            for (int e = 0; e < 8; ++e) h[e] *= w[e];
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) h[e] = WHOLE || e < have ? h[e] * f.inv : 0.0f;
+        for (int e = 0; e < 8; ++e) h[e] = WHOLE || e < have ? h[e] * f.m : 0.0f;
         if (a.y) store8(a.y + i * a.ldy + k, have, h);
     }
     if (a.format < 0) return;
@@ -156,7 +164,7 @@ __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
         __syncthreads();
         ss = (part[0] + part[1]) + (part[2] + part[3]);
     }
-    const Factor f = row_factor(ss, a.d, a.eps);
+    const Factor f = row_factor(ss, a.d, a.eps, a.weight != nullptr);
     if (CH > 0) {
 #pragma unroll
         for (int c = 0; c < CH; ++c) {

@@ -187,6 +187,7 @@ int bts_mx_dequantize(bts_context *ctx, const uint8_t *codes, const uint8_t *sca
 /* Root-mean-square norm of rows, with the residual's addition and a quantised output:
  *   h = x + residual, rounded to `dtype` (h = x without a residual);   v = h / sqrt(mean(h^2) + eps) * weight
  * sum (nullable) = h; y (nullable) = v in `dtype`; codes / scales (both nullable) = v in `format`, quantised from float32.
+ * h / sqrt(.) is held in float32: elements below 2^-126 of their row's norm lose digits, whatever their weight.
  * residual[n,d] and weight[d] are nullable, all of x's type.  sum and y may be x or residual themselves (same row stride), not
  * each other.  eps: a positive finite float32. */
 int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void *residual, int ldr,

@@ -296,6 +296,42 @@ def test_rms_norm_at_the_ends_of_the_range(bts, d, dtype):
         check_quantized(want, *host(q), "e4m3", d, delta)
 
 
+@pytest.mark.parametrize("d", [40, 1500, 1111, 9000])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_rms_norm_weights_at_the_ends_of_the_range(bts, d, dtype):
+    """rows and weights whose products leave float32 although the normalised values do not, in both directions, and elements far below
+    their row's norm.  The bound: half of the sum of squares' error (a square, and the three additions to eight of them, in float32:
+    4 roundings), the factor's rounding, the weight's product and the factor's product -- 5 roundings, and the output's.  Below float32's
+    normal range: the normalised element but for a factor in [1, 2) is held in float32, 2^-150 off, which the weight and that factor multiply;
+    the product with the weight likewise, 2^-150 times that factor."""
+    t, r = DTYPES[dtype], np.random.default_rng(d)
+    scale = np.array([50, 100, 126, 64, 0, -40, -62, -100, -118, 20])
+    x = (1 + r.random((len(scale), d))) * np.exp2(scale[:, None] * 1.0) * r.choice([-1, 1], (len(scale), d))
+    x[3, ::3] *= 2.0 ** -100                                                         # 2^-36 beside 2^64
+    x[2, ::2] *= 2.0 ** -180
+    x[9] = 0
+    x = torch.from_numpy(x).to(t)
+    for power in (100, 64, 30, 0, -30, -64, -95):
+        w = torch.from_numpy((1 + r.random(d)) * np.exp2(power - 1.0) * r.choice([-1, 1], d)).to(t)
+        w[5] = 0
+        for eps in (1e-38, 1e-6):
+            y = torch.empty_like(x).cuda()
+            q, _ = bts.rms_norm_mx(x.cuda(), weight=w.cuda(), eps=eps, y_out=y)
+            _, want = norm_ref(x, None, w, eps)
+            delta = 5.01 * 2.0 ** -24
+            tiny = float(torch.finfo(t).smallest_normal)
+            wide_w = np.abs(w.double().numpy())
+            tol = (delta + HALF[dtype] * (1 + delta)) * np.abs(want) + tiny * HALF[dtype] + 2.0 ** -149 + 2.0 ** -149 * wide_w
+            got = y.cpu().double().numpy()
+            assert (np.abs(got - want) <= tol).all(), (power, eps, float((np.abs(got - want) / tol).max()))
+            # (a value below float32's normal range is rounded to its smallest step before it is quantised: blocks of such are left out)
+            ok = (np.abs(blocks(want, d)).max(-1) >= 2.0 ** -100) | (np.abs(blocks(want, d)).max(-1) == 0)
+            code, s = host(q)
+            code = code.reshape(len(x), -1, 32)
+            code[~ok], s[~ok] = 0, 0
+            check_quantized(np.where(ok[:, :, None], blocks(want, d), 0).reshape(len(x), -1)[:, :d], code.reshape(len(x), -1), s, "e4m3", d, delta)
+
+
 # more rows than one launch's workgroups, 4 rows each up to 1024 elements
 @pytest.mark.parametrize("n,d", [(4 * 2 ** 20 + 5, 8), (2 ** 20 + 3, 1032)])
 def test_rms_norm_big_row_counts(bts, n, d):
@@ -319,6 +355,18 @@ def test_rms_norm_zero_and_non_finite_rows(bts):
     assert (v[0] == 0.875).all() and (v[4] == 0.875).all() and (v[1] == 0).all()
     assert np.isnan(v[3]).all()                                                     # a NaN takes the row's norm with it
     assert np.isnan(v[2, :32]).all() and (v[2, 32:] == 0).all()                     # inf / inf in its block, x / inf elsewhere
+
+
+@pytest.mark.parametrize("power", [100, 0, -100])
+def test_rms_norm_non_finite_rows_under_a_weight(bts, power):
+    x = torch.ones((3, 300)) * 2.0 ** 50
+    x[0, 7] = float("inf"); x[1, 70] = float("nan")
+    w = torch.ones(300) * 2.0 ** power
+    y = torch.empty_like(x).cuda()
+    bts.rms_norm_mx(x.cuda(), weight=w.cuda(), fmt=None, y_out=y)
+    y = y.cpu()
+    assert y[0, 7].isnan() and (y[0, :7] == 0).all() and (y[0, 8:] == 0).all() and y[1].isnan().all()
+    assert (y[2] == 2.0 ** power).all()                                              # sqrt(2^100 + 1e-6) = 2^50 in float64
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
