@@ -13,17 +13,20 @@ from . import _lib
 torch = None                            # imported by the first call: importing the package does not
 _DTYPES = {}                            # enum bts_dtype
 _raw_stream = None
+_forward_ad = None
 _FORMATS = {"e2m1": 0, "e4m3": 1}       # enum bts_mx_format
 _ROW, _BLOCK = 128, 32                  # elements a row is padded to; elements per scale
 _MOST = 0x7fffffff                      # rows and row strides are C ints
 
 
 def _init():
-    global torch, _raw_stream
+    global torch, _raw_stream, _forward_ad
     import torch as t
+    from torch.autograd import forward_ad
     _DTYPES.update({t.float32: 1, t.float16: 2, t.bfloat16: 3})
     # the number of a device's current stream without the Stream object around it (2 us of a 10 us call)
     _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None)
+    _forward_ad = forward_ad
     torch = t
 
 
@@ -51,14 +54,21 @@ def _width(d):
     return (d + _ROW - 1) // _ROW * _ROW
 
 
+def _no_gradient(t, name):
+    if t.requires_grad and torch.is_grad_enabled():
+        raise _lib.BtsError("%s: no gradient is formed here: detach it or call under torch.no_grad()" % name)
+    # (unpack_dual takes 0.3 us a tensor: only inside a dual_level)
+    if getattr(_forward_ad, "_current_level", 0) >= 0 and _forward_ad.unpack_dual(t).tangent is not None:
+        raise _lib.BtsError("%s: no tangent is formed here: unpack the dual tensor" % name)
+
+
 def _rows2d(t, name, like=None):
     """A device matrix with unit column stride -> (pointer, row stride in elements)."""
     if not t.is_cuda:
         raise _lib.BtsError("%s: a device tensor is expected" % name)
     if t.dim() != 2:
         raise _lib.BtsError("%s: [rows, d] expected, got %d dimensions" % (name, t.dim()))
-    if t.requires_grad and torch.is_grad_enabled():
-        raise _lib.BtsError("%s: no gradient is formed here: detach it or call under torch.no_grad()" % name)
+    _no_gradient(t, name)
     n, d = t.shape
     ld, unit = t.stride()
     if n <= 1:
@@ -205,8 +215,8 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     pr, ldr = _rows2d(residual, "residual", x) if residual is not None else (None, 0)
     if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous()):
         raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
-    if weight is not None and weight.requires_grad and torch.is_grad_enabled():
-        raise _lib.BtsError("weight: no gradient is formed here: detach it or call under torch.no_grad()")
+    if weight is not None:
+        _no_gradient(weight, "weight")
     py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
     if sum_out is None and (residual is not None or py == px):      # (y in the place of x: h is x as it was)
         sum_out = torch.empty((n, d), dtype=x.dtype, device=x.device)

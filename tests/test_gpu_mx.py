@@ -575,6 +575,24 @@ def test_leaves_that_want_a_gradient(bts):
         assert len(bts.mx_quantize(x)) == 2 and len(bts.rms_norm_mx(x, weight=w)[0]) == 2
 
 
+@pytest.mark.skipif("libbotsort_emu" in __import__("os").environ.get("BTS_LIB_PATH", ""), reason="torch's dual tensors need the functions that the emulation replaces")
+def test_forward_mode_tangents_are_refused(bts):
+    """a dual tensor's tangent would be dropped without a word; while gradients are off too, forward mode goes on there"""
+    from torch.autograd import forward_ad
+    x, w = torch.ones((2, 64)).cuda(), torch.ones(64).cuda()
+    with forward_ad.dual_level():
+        dx, dw = forward_ad.make_dual(x, x), forward_ad.make_dual(w, w)
+        calls = (lambda: bts.mx_quantize(dx), lambda: bts.rms_norm_mx(dx), lambda: bts.rms_norm_mx(x, weight=dw), lambda: bts.rms_norm_mx(x, residual=dx),
+                 lambda: bts.rms_norm_mx(x, sum_out=dx), lambda: bts.mx_product(bts.mx_quantize(x), bts.mx_quantize(x), out=dx[:, :2]))
+        for call in calls:
+            with pytest.raises(bts.BtsError):
+                call()
+            with torch.no_grad(), pytest.raises(bts.BtsError):
+                call()
+        assert len(bts.rms_norm_mx(x, weight=w)[0]) == 2
+    assert len(bts.mx_quantize(x)) == 2
+
+
 def test_two_runs_give_the_same_bits(bts):
     a, _ = rows_of(bts, feature_rows(150, 900, 7), "e4m3")
     b, _ = rows_of(bts, feature_rows(90, 900, 8), "e2m1")

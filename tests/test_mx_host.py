@@ -20,3 +20,16 @@ def test_host_tensors_are_refused():
     for call in (lambda: bts.mx_quantize(torch.ones(4, 64)), lambda: bts.rms_norm_mx(torch.ones(4, 64))):
         with pytest.raises(bts.BtsError):
             call()
+
+
+def test_forward_mode_tangents_are_refused(monkeypatch):
+    from torch.autograd import forward_ad
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    x, w = torch.ones(2, 64), torch.ones(64)
+    with forward_ad.dual_level():
+        dx, dw = forward_ad.make_dual(x, x), forward_ad.make_dual(w, w)
+        for call in (lambda: bts.mx_quantize(dx), lambda: bts.rms_norm_mx(dx), lambda: bts.rms_norm_mx(x, residual=dx), lambda: bts.rms_norm_mx(x, weight=dw)):
+            with pytest.raises(bts.BtsError, match="tangent"):
+                call()
+            with torch.no_grad(), pytest.raises(bts.BtsError, match="tangent"):       # (forward mode goes on there)
+                call()
