@@ -13,20 +13,21 @@ from . import _lib
 torch = None                            # imported by the first call: importing the package does not
 _DTYPES = {}                            # enum bts_dtype
 _raw_stream = None
-_forward_ad = None
+_forward_ad = _increment_version = None
 _FORMATS = {"e2m1": 0, "e4m3": 1}       # enum bts_mx_format
 _ROW, _BLOCK = 128, 32                  # elements a row is padded to; elements per scale
 _MOST = 0x7fffffff                      # rows and row strides are C ints
 
 
 def _init():
-    global torch, _raw_stream, _forward_ad
+    global torch, _raw_stream, _forward_ad, _increment_version
     import torch as t
     from torch.autograd import forward_ad
+    from torch.autograd.graph import increment_version
     _DTYPES.update({t.float32: 1, t.float16: 2, t.bfloat16: 3})
     # the number of a device's current stream without the Stream object around it (2 us of a 10 us call)
     _raw_stream = getattr(t._C, "_cuda_getCurrentRawStream", None)
-    _forward_ad = forward_ad
+    _forward_ad, _increment_version = forward_ad, increment_version
     torch = t
 
 
@@ -183,6 +184,13 @@ class MxRows:
         return out
 
 
+def _written(*given):
+    """Matrices and rows that the caller handed in to be filled (or None): autograd's check of saved tensors is to see that they changed."""
+    for t in given:
+        if t is not None:
+            _increment_version(t if not isinstance(t, MxRows) else t._room if t._room is not None else (t._codes, t._scales))
+
+
 def _room(out, n, d, fmt, device):
     if out is None:
         return MxRows.empty(n, d, fmt, device)
@@ -196,11 +204,12 @@ def mx_quantize(x, fmt: str = "e2m1", out: MxRows = None) -> MxRows:
     dt, f = _dtype_code(x.dtype), _format_code(fmt)
     p, ld = _rows2d(x, "x")
     n, d = x.shape
-    out = _room(out, n, d, fmt, x.device)
+    rows = _room(out, n, d, fmt, x.device)
     lib, ctx, stream = _call(x.device)
-    pc, ps = out._pointers()
+    pc, ps = rows._pointers()
     _lib.check(lib.bts_mx_quantize(ctx, p, dt, ld, n, d, f, pc, ps, stream))
-    return out
+    _written(out)
+    return rows
 
 
 def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4m3", sum_out=None, y_out=None, out: MxRows = None):
@@ -218,9 +227,10 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     if weight is not None:
         _no_gradient(weight, "weight")
     py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
-    if sum_out is None and (residual is not None or py == px):      # (y in the place of x: h is x as it was)
-        sum_out = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    ps, lds = _rows2d(sum_out, "sum_out", x) if sum_out is not None else (None, 0)
+    h = sum_out
+    if h is None and (residual is not None or py == px):            # (y in the place of x: h is x as it was)
+        h = torch.empty((n, d), dtype=x.dtype, device=x.device)
+    ps, lds = _rows2d(h, "sum_out", x) if h is not None else (None, 0)
     if fmt is None and out is not None:
         raise _lib.BtsError("out: rows to fill need their fmt")
     f = 0 if fmt is None else _format_code(fmt)
@@ -229,7 +239,8 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     qc, qs = (None, None) if rows is None else rows._pointers()
     _lib.check(lib.bts_rms_norm(ctx, dt, px, ldx, pr, ldr, None if weight is None else weight.data_ptr(), n, d, float(eps), ps, lds, py, ldy, f,
                                 qc, qs, stream))
-    return rows, x if sum_out is None else sum_out
+    _written(sum_out, y_out, out)
+    return rows, x if h is None else h
 
 
 def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = False, dtype=None, out=None):
@@ -243,6 +254,7 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
     if a.d != b.d or b.device != device:
         raise _lib.BtsError("mx_product: rows of one width on one device expected, got %r and %r" % (a, b))
     n, m = a._n, b._n
+    given = out
     if out is None:
         if dtype is None:
             dtype = torch.float32 if a.fmt == b.fmt == "e2m1" else torch.bfloat16
@@ -256,4 +268,5 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
     lib, ctx, stream = _call(device)
     (ac, as_), (bc, bs) = a._pointers(), b._pointers()
     _lib.check(lib.bts_mx_product(ctx, ac, as_, a._code, n, bc, bs, b._code, m, a.d, float(alpha), 1 if floor_zero else 0, po, code, ld, stream))
+    _written(given)
     return out

@@ -593,6 +593,35 @@ def test_forward_mode_tangents_are_refused(bts):
     assert len(bts.mx_quantize(x)) == 2
 
 
+def test_what_is_written_in_place_counts_as_changed(bts):
+    """autograd's check of saved tensors: an output in the place of a tensor that a backward pass needs makes that pass an error"""
+    leaf = torch.linspace(-1, 1, 128).view(2, 64).cuda().requires_grad_()
+    saved = leaf.exp()                                                              # (exp keeps its result for the backward pass)
+    with torch.no_grad():
+        bts.rms_norm_mx(saved, residual=torch.ones_like(saved), sum_out=saved)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        saved.sum().backward()
+    x, h, y = (torch.ones((3, 64)).cuda() for _ in range(3))
+    rows, own = bts.MxRows.empty(3, 64, "e4m3"), bts.mx_quantize(x)
+    part = bts.MxRows(rows.codes, rows.scales, 64, "e4m3")
+    out = torch.zeros((3, 3), dtype=torch.bfloat16).cuda()
+    for written, call in (((h, y, rows.codes, rows.scales), lambda: bts.rms_norm_mx(x, sum_out=h, y_out=y, out=rows)), ((x,), lambda: bts.rms_norm_mx(x, y_out=x)),
+                          ((part.codes, part.scales, rows.codes), lambda: bts.mx_quantize(x, "e4m3", out=part)), ((out,), lambda: bts.mx_product(own, own, out=out))):
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > b for t, b in zip(written, before))
+    before = x._version, own.codes._version
+    bts.rms_norm_mx(x, residual=h)
+    bts.mx_product(own, own)
+    own.dequantize()
+    assert (x._version, own.codes._version) == before                              # (what is only read does not)
+    with torch.inference_mode():                                                    # (tensors without a counter)
+        z = torch.ones((3, 64)).cuda()
+        assert bts.rms_norm_mx(z, y_out=z, out=bts.MxRows.empty(3, 64, "e4m3"))[1].shape == (3, 64)
+    with torch.no_grad():
+        bts.rms_norm_mx(x, sum_out=z, y_out=y)
+
+
 def test_two_runs_give_the_same_bits(bts):
     a, _ = rows_of(bts, feature_rows(150, 900, 7), "e4m3")
     b, _ = rows_of(bts, feature_rows(90, 900, 8), "e2m1")
