@@ -31,6 +31,14 @@ def _init():
     torch = t
 
 
+def _tensor(t, name):
+    if torch is None:
+        _init()
+    if not isinstance(t, torch.Tensor):
+        raise _lib.BtsError("%s: a device tensor is expected, got %s" % (name, type(t).__name__))
+    return t
+
+
 def _dtype_code(dtype):
     if torch is None:
         _init()
@@ -65,7 +73,7 @@ def _no_gradient(t, name):
 
 def _rows2d(t, name, like=None):
     """A device matrix with unit column stride -> (pointer, row stride in elements)."""
-    if not t.is_cuda:
+    if not _tensor(t, name).is_cuda:
         raise _lib.BtsError("%s: a device tensor is expected" % name)
     if t.dim() != 2:
         raise _lib.BtsError("%s: [rows, d] expected, got %d dimensions" % (name, t.dim()))
@@ -108,8 +116,7 @@ class MxRows:
     __slots__ = ("d", "fmt", "device", "_code", "_n", "_room", "_codes", "_scales")
 
     def __init__(self, codes, scales, d: int, fmt: str):
-        if torch is None:
-            _init()
+        _tensor(codes, "codes"), _tensor(scales, "scales")
         self._code = _format_code(fmt)
         d, wide = int(d), _width(d)
         n = codes.shape[0] if codes.dim() == 2 and codes.shape[0] <= _MOST else -1
@@ -194,6 +201,8 @@ def _written(*given):
 def _room(out, n, d, fmt, device):
     if out is None:
         return MxRows.empty(n, d, fmt, device)
+    if not isinstance(out, MxRows):
+        raise _lib.BtsError("out: MxRows expected, got %s" % type(out).__name__)
     if out._n != n or out.d != d or out.fmt != fmt or out.device != device:
         raise _lib.BtsError("out: %d x %d rows in %s on %s expected, got %r" % (n, d, fmt, device, out))
     return out
@@ -201,7 +210,7 @@ def _room(out, n, d, fmt, device):
 
 def mx_quantize(x, fmt: str = "e2m1", out: MxRows = None) -> MxRows:
     """x [n, d] (float32, float16 or bfloat16; rows may be strided) -> its rows in 4 (e2m1) or 8 (e4m3) bits; `out`: rows to fill."""
-    dt, f = _dtype_code(x.dtype), _format_code(fmt)
+    dt, f = _dtype_code(_tensor(x, "x").dtype), _format_code(fmt)
     p, ld = _rows2d(x, "x")
     n, d = x.shape
     rows = _room(out, n, d, fmt, x.device)
@@ -218,13 +227,13 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
 
     `sum_out` (may be x or residual themselves: the addition in place) receives h, `y_out` (likewise) the normalised rows in x's type.
     Without a residual h is x itself, or a copy where y_out takes its place."""
-    dt = _dtype_code(x.dtype)
+    dt = _dtype_code(_tensor(x, "x").dtype)
     px, ldx = _rows2d(x, "x")
     n, d = x.shape
     pr, ldr = _rows2d(residual, "residual", x) if residual is not None else (None, 0)
-    if weight is not None and (weight.shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous()):
-        raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
     if weight is not None:
+        if _tensor(weight, "weight").shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous():
+            raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
         _no_gradient(weight, "weight")
     py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
     h = sum_out
@@ -261,7 +270,7 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
         code = _dtype_code(dtype)
         out = torch.empty((n, m), dtype=dtype, device=device)
     else:
-        code = _dtype_code(out.dtype)
+        code = _dtype_code(_tensor(out, "out").dtype)
         if tuple(out.shape) != (n, m) or out.device != device or dtype not in (None, out.dtype):
             raise _lib.BtsError("out: [%d, %d] on %s%s expected" % (n, m, device, "" if dtype is None else " of %s" % dtype))
     po, ld = _rows2d(out, "out")

@@ -33,3 +33,19 @@ def test_forward_mode_tangents_are_refused(monkeypatch):
                 call()
             with torch.no_grad(), pytest.raises(bts.BtsError, match="tangent"):       # (forward mode goes on there)
                 call()
+
+
+def test_what_is_not_a_tensor_is_refused_by_name(monkeypatch):
+    """lists, arrays and rows of another kind: the package's error, saying which argument"""
+    import numpy as np
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    x, rows, a = torch.ones(2, 64), bts.MxRows.empty(2, 64, "e4m3", device="cpu"), np.ones((2, 64), np.float32)
+    for name, call in (("x", lambda: bts.mx_quantize([[1.0] * 64])), ("x", lambda: bts.mx_quantize(a)), ("x", lambda: bts.rms_norm_mx(a)), ("x", lambda: bts.mx_quantize(None)),
+                       ("out", lambda: bts.mx_quantize(x, "e4m3", out=x)), ("out", lambda: bts.rms_norm_mx(x, out=torch.ones(2, 64))),
+                       ("residual", lambda: bts.rms_norm_mx(x, residual=a)), ("weight", lambda: bts.rms_norm_mx(x, weight=a[0])),
+                       ("weight", lambda: bts.rms_norm_mx(x, weight=[1.0] * 64)), ("sum_out", lambda: bts.rms_norm_mx(x, sum_out=a)),
+                       ("y_out", lambda: bts.rms_norm_mx(x, y_out=rows)), ("out", lambda: bts.mx_product(rows, rows, out=a)),
+                       ("out", lambda: bts.mx_product(rows, rows, out=rows)), ("MxRows", lambda: bts.mx_product(rows, x)),
+                       ("codes", lambda: bts.MxRows(np.zeros((2, 128), np.uint8), rows.scales, 64, "e4m3")), ("scales", lambda: bts.MxRows(rows.codes, None, 64, "e4m3"))):
+        with pytest.raises(bts.BtsError, match=name):
+            call()
