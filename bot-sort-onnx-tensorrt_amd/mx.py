@@ -71,6 +71,12 @@ def _no_gradient(t, name):
         raise _lib.BtsError("%s: no tangent is formed here: unpack the dual tensor" % name)
 
 
+def _no_negative(t, name):
+    # (parts of complex tensors have a stride of 2: they get here as single columns only)
+    if t.is_neg():
+        raise _lib.BtsError("%s: the imaginary part of a conjugate: call .resolve_neg()" % name)
+
+
 def _rows2d(t, name, like=None):
     """A device matrix with unit column stride -> (pointer, row stride in elements)."""
     if not _tensor(t, name).is_cuda:
@@ -84,6 +90,8 @@ def _rows2d(t, name, like=None):
         ld = max(d, 1)
     if (unit != 1 and d > 1) or ld < d:
         raise _lib.BtsError("%s: the elements of a row must be adjacent and rows may not overlap (strides %s): call .contiguous()" % (name, t.stride()))
+    if unit != 1:
+        _no_negative(t, name)
     if n > _MOST or ld > _MOST:
         raise _lib.BtsError("%s: at most 2^31 - 1 rows, and elements between them" % name)
     if like is not None and (t.shape != like.shape or t.dtype != like.dtype or t.device != like.device):
@@ -235,6 +243,8 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
         if _tensor(weight, "weight").shape != (d,) or weight.dtype != x.dtype or weight.device != x.device or not weight.is_contiguous():
             raise _lib.BtsError("weight: contiguous [%d] of x's type and device expected" % d)
         _no_gradient(weight, "weight")
+        if d == 1:
+            _no_negative(weight, "weight")
     py, ldy = _rows2d(y_out, "y_out", x) if y_out is not None else (None, 0)
     h = sum_out
     if h is None and (residual is not None or py == px):            # (y in the place of x: h is x as it was)

@@ -49,3 +49,13 @@ def test_what_is_not_a_tensor_is_refused_by_name(monkeypatch):
                        ("codes", lambda: bts.MxRows(np.zeros((2, 128), np.uint8), rows.scales, 64, "e4m3")), ("scales", lambda: bts.MxRows(rows.codes, None, 64, "e4m3"))):
         with pytest.raises(bts.BtsError, match=name):
             call()
+
+
+def test_views_that_hold_the_negative_are_refused(monkeypatch):
+    """the imaginary part of a conjugate is a view whose memory holds the other sign: one column of it has rows like any matrix's"""
+    monkeypatch.setattr(torch.Tensor, "is_cuda", property(lambda self: True))
+    z = torch.complex(torch.ones(4, 1), torch.ones(4, 1)).conj().imag
+    assert z.is_neg() and (z == -1).all()
+    for call in (lambda: bts.mx_quantize(z), lambda: bts.rms_norm_mx(z), lambda: bts.rms_norm_mx(torch.ones(4, 1), weight=z[0])):
+        with pytest.raises(bts.BtsError, match="conjugate"):
+            call()
