@@ -783,6 +783,7 @@ int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_sc
     BTS_REQUIRE(known_format(a_format) && known_format(b_format) && known_dtype(out_dtype), "unknown format / type");
     BTS_REQUIRE(out_dtype != BTS_F32 || (a_format == E2M1 && b_format == E2M1),
                 "a float32 output needs two E2M1 operands (products with an E4M3 operand carry about 16 bits)");
+    BTS_REQUIRE(fabs(alpha) <= 3.4028234663852886e38 && ((float)alpha != 0.0f || alpha == 0.0), "alpha must be a float32: finite, and not too small for one");
     BTS_ON_DEVICE(ctx);
     if (n == 0 || m == 0) return BTS_OK;
     BTS_REQUIRE(a_codes && a_scales && b_codes && b_scales && out, "null pointer");

@@ -194,7 +194,7 @@ int bts_rms_norm(bts_context *ctx, int dtype, const void *x, int ldx, const void
                  const void *weight, int n, int d, double eps, void *sum, int lds, void *y, int ldy,
                  int format, uint8_t *codes, uint8_t *scales, bts_stream stream);
 
-/* out[i*ld+j] = alpha * <a_i, b_j>, optionally max(0, .) (floor_zero != 0; a NaN stays one): bts_cos_similarity on microscaled
+/* out[i*ld+j] = (float) alpha * <a_i, b_j>, optionally max(0, .) (floor_zero != 0; a NaN stays one): bts_cos_similarity on microscaled
  * rows.  a: n rows, b: m rows, of the same d; formats may differ.  Products are formed exactly and added in float32 where both are
  * E2M1; the matrix instruction aligns the products of an E4M3 operand to the largest of them with about 13 bits behind it, so
  * out_dtype BTS_F32 needs two E2M1 operands and the 16-bit types take any. */

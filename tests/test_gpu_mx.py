@@ -771,6 +771,17 @@ def test_overlapping_tensors_are_refused(bts):
     assert bts.mx_product(q, q).shape == (6, 6)
 
 
+def test_factors_that_float32_does_not_hold(bts):
+    """the kernels multiply by alpha in float32: 1e300 would be infinite and 1e-60 nothing, whatever the products are"""
+    v = torch.ones((2, 64)).cuda()
+    q = bts.mx_quantize(v)
+    for alpha in (1e300, -1e39, 1e-60, float("inf"), float("-inf"), float("nan")):
+        with pytest.raises(bts.BtsError, match="alpha"):
+            bts.mx_product(q, q, alpha=alpha)
+    for alpha in (0.0, -0.0, 1e-44, 2.0 ** -126, -5.3e36):                           # (64 times these: exact)
+        assert (bts.mx_product(q, q, alpha=alpha).cpu() == 64 * torch.tensor(alpha, dtype=torch.float32)).all()
+
+
 # ------------------------------------------------------------------------------------------- streams, graphs, threads (hardware)
 
 @pytest.mark.skipif("libbotsort_emu" in __import__("os").environ.get("BTS_LIB_PATH", ""), reason="needs real streams and graphs")
