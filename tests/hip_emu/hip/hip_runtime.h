@@ -362,7 +362,7 @@ static inline hipError_t hipGetDevice(int *d) { *d = 0; return hipSuccess; }
 static inline hipError_t hipSetDevice(int) { return hipSuccess; }
 namespace emu { void drain_all(); }
 static inline hipError_t hipDeviceSynchronize() { emu::drain_all(); return hipSuccess; }
-static inline hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) { memset(p, 0, sizeof(*p)); strcpy(p->name, "CPU emulation of gfx950"); strcpy(p->gcnArchName, "gfx950:sramecc+:xnack-"); p->multiProcessorCount = 256; p->totalGlobalMem = (size_t)1 << 34; return hipSuccess; }
+static inline hipError_t hipGetDeviceProperties(hipDeviceProp_t *p, int) { memset(p, 0, sizeof(*p)); strcpy(p->name, "CPU emulation of gfx950"); strcpy(p->gcnArchName, "gfx950:sramecc+:xnack-"); const char *cus = getenv("HIPEMU_CUS"); p->multiProcessorCount = cus ? atoi(cus) : 256; p->totalGlobalMem = (size_t)1 << 34; return hipSuccess; }
 static inline hipError_t hipMalloc(void **p, size_t n) { *p = aligned_alloc(256, (n + 255) / 256 * 256); return *p ? hipSuccess : hipErrorOutOfMemory; }
 static inline hipError_t hipFree(void *p) { emu::drain_all(); free(p); return hipSuccess; }
 static inline hipError_t hipHostMalloc(void **p, size_t n, unsigned = 0) { return hipMalloc(p, n); }

@@ -243,6 +243,41 @@ def test_rms_norm(bts, n, d, dtype, residual, weight):
             check_quantized(v, *host(q), fmt, d, delta)
 
 
+@pytest.mark.parametrize("residual,weight", [(False, False), (True, True)])
+@pytest.mark.parametrize("dtype", list(DTYPES))
+@pytest.mark.parametrize("n,d", NORM_SHAPES)
+def test_rms_norm_error_does_not_grow_with_the_row(bts, n, d, dtype, residual, weight):
+    """as `test_rms_norm`, with the bound of what is computed: eight squares are added in float32 (a square and three additions, half of whose
+    4 roundings reach the root), the rest of the row in float64; the factor, the weight's product and the factor's product are rounded
+    once each -- 5 roundings whatever the row's length"""
+    t, r = DTYPES[dtype], np.random.default_rng(d + 1)
+    x = torch.from_numpy(r.standard_normal((n, d)) * np.exp2(r.integers(-4, 5, (n, 1)))).to(t)
+    res = torch.from_numpy(r.standard_normal((n, d))).to(t) if residual else None
+    w = torch.from_numpy(1 + 0.2 * r.standard_normal(d)).to(t) if weight else None
+    dev = lambda a: None if a is None else a.cuda()  # noqa: E731
+    delta = 5.01 * 2.0 ** -24
+    for fmt in ("e4m3", "e2m1"):
+        y = torch.full((n, d), 9.0, dtype=t).cuda()
+        q, h = bts.rms_norm_mx(x.cuda(), residual=dev(res), weight=dev(w), eps=1e-5, fmt=fmt, y_out=y)
+        want_h, v = norm_ref(x, res, w, 1e-5)
+        assert torch.equal(h.cpu(), want_h)
+        tol = (delta + HALF[dtype] * (1 + delta)) * np.abs(v) + float(torch.finfo(t).smallest_normal) * HALF[dtype]
+        assert (np.abs(y.cpu().double().numpy() - v) <= tol).all()
+        check_quantized(v, *host(q), fmt, d, delta)
+
+
+@pytest.mark.parametrize("n,d", [(64, 2048), (64, 1111), (64, 8192), (64, 9000), (64, 512)])
+def test_rms_norm_factor_is_rounded_once(bts, n, d):
+    """whole numbers up to 511: eight squares add up exactly in float32 (below 2^21), a row's do not (around 2^26 at 1111 elements), so
+    only a sum in more bits gives the factor that float64 gives, and with it every bit of y"""
+    r = np.random.default_rng(d)
+    x = r.integers(-511, 512, (n, d)).astype(np.float64)
+    y = torch.empty((n, d)).cuda()
+    bts.rms_norm_mx(torch.from_numpy(x).float().cuda(), eps=1e-6, fmt=None, y_out=y)
+    factor = (1.0 / np.sqrt((x * x).sum(1) / d + 1e-6)).astype(np.float32)
+    assert np.array_equal(y.cpu().numpy(), x.astype(np.float32) * factor[:, None])
+
+
 @pytest.mark.parametrize("d", [96, 5000, 9000])
 def test_rms_norm_in_place(bts, d):
     x = awkward(6, d, "bf16", d)
@@ -443,6 +478,60 @@ def test_product_tiles(bts, n, m, d, fa, fb):
 @pytest.mark.parametrize("n,m,d", BIG)
 def test_product_big(bts, n, m, d, fa, fb):
     run_product(bts, n, m, d, fa, fb, "f32" if fa == fb == "e2m1" else "bf16")
+
+
+def random_rows(bts, n, d, fmt, seed):
+    """rows of random codes (no NaN) and scales 2^-5 .. 2^5, d even -> (MxRows, their values in float64, on the device)"""
+    r = np.random.default_rng(seed)
+    code = r.integers(0, 256, (n, wide(d) // (2 if fmt == "e2m1" else 1)), dtype=np.uint8)
+    if fmt == "e4m3":
+        code[code % 128 == 127] = 1
+    code[:, d // (2 if fmt == "e2m1" else 1):] = 0
+    s = r.integers(122, 133, (n, wide(d) // 32), dtype=np.uint8)
+    g = torch.from_numpy(grid(fmt)).cuda()
+    table = torch.cat((g, -g)) if fmt == "e2m1" else torch.cat((g, g[:1], -g, g[:1]))
+    code, s = torch.from_numpy(code).cuda(), torch.from_numpy(s).cuda()
+    c = code.long() if fmt == "e4m3" else torch.stack((code & 15, code >> 4), -1).view(n, -1).long()
+    return bts.MxRows(code, s, d, fmt), table[c] * torch.exp2(s.double() - 127).repeat_interleave(32, 1)
+
+
+# The 256 x 256 and 128 x 128 tiles, from one stage to an odd and an even number of many.  The large sizes select them on a card of 256
+# CUs, the small ones on the emulation told to have one.
+LARGE_TILES = [pytest.param(n, m, d, id="%s-%d-%d-%d" % (name, n, m, d))
+               for name, n, m, depths in (("big256", 4000, 4090, (100, 2048, 2176, 2300)), ("big128", 2900, 2970, (100, 2048, 2176, 2300)),
+                                          ("one256", 200, 250, (100, 768, 898)), ("four256", 300, 500, (100, 640)), ("few128", 100, 300, (100, 384, 640, 768)))
+               for d in depths]
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m,d", LARGE_TILES)
+def test_product_large_tiles(bts, n, m, d, fa, fb):
+    """the sum's own error is `product_bound`'s, times the factor"""
+    (a, ra), (b, rb) = random_rows(bts, n, d, fa, n + d), random_rows(bts, m, d, fb, m + d + 1)
+    rbt = rb.t().contiguous()
+    ref, mag = ra @ rbt, ra.abs() @ rbt.abs()
+    own = (wide(d) / 128 + 20) * 2.0 ** -24 if fa == fb == "e2m1" else 2.0 ** -12
+    for out, alpha, floor in (("f32" if fa == fb == "e2m1" else "bf16", -0.75, False), ("bf16", 0.125, True)):
+        want = (ref * alpha).clamp(min=0) if floor else ref * alpha
+        got = bts.mx_product(a, b, alpha=alpha, floor_zero=floor, dtype=DTYPES[out]).double()
+        tol = HALF[out] * want.abs() + own * abs(alpha) * mag + float(torch.finfo(DTYPES[out]).smallest_normal) * HALF[out]
+        assert ((got - want).abs() <= tol).all(), float(((got - want).abs() / tol).max())
+
+
+@pytest.mark.parametrize("fa,fb", FMTS)
+@pytest.mark.parametrize("n,m,d", PRODUCTS + [(512, 256, 256)])
+def test_product_error_goes_with_the_factor(bts, n, m, d, fa, fb):
+    """as `run_product`, with the sum's own error times the factor for every type of output"""
+    a, ra = rows_of(bts, feature_rows(n, d, 7 * n + d), fa)
+    b, rb = rows_of(bts, feature_rows(m, d, 9 * m + d), fb)
+    ref, mag = ra @ rb.T, np.abs(ra) @ np.abs(rb).T
+    own = (d / 128 + 20) * 2.0 ** -24 if fa == fb == "e2m1" else 2.0 ** -12
+    for out in ("f32", "bf16", "f16") if fa == fb == "e2m1" else ("f16", "bf16"):
+        for alpha in (0.125, -0.0437):
+            got = bts.mx_product(a, b, alpha=alpha, dtype=DTYPES[out]).cpu().double().numpy()
+            want = ref * float(np.float32(alpha))
+            tol = HALF[out] * np.abs(want) + own * abs(alpha) * mag + float(torch.finfo(DTYPES[out]).smallest_normal) * HALF[out]
+            assert (np.abs(got - want) <= tol).all(), (out, alpha)
 
 
 def test_product_big_row_counts(bts):
