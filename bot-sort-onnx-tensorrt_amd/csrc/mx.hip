@@ -420,10 +420,11 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
 // the writes to LDS 25 more, the loads 28; the reads cost nothing beside the instructions.  A round of tiles computes and then stores together, so the output of
 // 10000 x 2000 float32 (17 us) comes on top of the loop (14 us per 1024 elements of depth).  256 x 256 tiles of E4M3 x E2M1, 16384 x 8192 x
 // 4096: 440 us, 2.5 PFLOP/s; the same with zeros in all codes is a quarter faster, that is the card's power limit.
-template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD>
+template <int FA, int FB, int TM, int TN, int WM, int WN, int SK>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     constexpr int THREADS = 64 * WM * WN, RT = TM / WM / 16, CT = TN / WN / 16;
     constexpr bool PHASED = WM * WN == 8;
+    constexpr int AHEAD = PHASED ? 1 : 2;
     typedef Operand<FA, TM, THREADS, SK> OpA;
     typedef Operand<FB, TN, THREADS, SK> OpB;
     static_assert((RT % 4 == 0 || TM <= 64) && (CT % 4 == 0 || TN <= 64), "scale bytes come four fragments to a word");
@@ -498,14 +499,14 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
 #pragma unroll
             for (int u = 0; u < RT; ++u) acc[u][w] = mma_bytes<FA, FB>(f.b[w], f.a[u], acc[u][w], f.sb[w / 4], w, f.sa[u / 4], u);
     };
-    Stage odd, even;                                         // (AHEAD 1: every stage goes through `odd`)
+    Stage odd, even;                                         // (PHASED: every stage goes through `odd`)
     load(odd, 0);
-    if (AHEAD == 2) load(even, 1);
+    if (!PHASED) load(even, 1);
     store(odd, 0);
     load(odd, AHEAD);
     __syncthreads();
     if constexpr (PHASED) {
-        static_assert(SK == 1 && AHEAD == 1, "one depth a stage");
+        static_assert(SK == 1, "one depth a stage");
         constexpr int READS = RT * OpA::S1 / 64 + CT * OpB::S1 / 64 + RT / 4 + CT / 4, LOADS = OpA::MOVES + OpB::MOVES + SMOVES;
         if (wave >= 4) __syncthreads();
         for (int t = 0; t < stages; ++t) {
@@ -545,10 +546,10 @@ __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
             }
         };
         for (int t = 0; t + 1 < stages; t += 2) {
-            step(t, AHEAD == 1 ? odd : even, 0);
+            step(t, even, 0);
             step(t + 1, odd, SK & 1);
         }
-        if (stages & 1) step(stages - 1, AHEAD == 1 ? odd : even, 0);
+        if (stages & 1) step(stages - 1, even, 0);
     }
     if (PHASED && wave < 4) __syncthreads();
     uint8_t *room = image + wave * 2048;
@@ -648,9 +649,9 @@ template <class Launch> void in_runs(ProductArgs &p, long tiles, Launch launch) 
         launch(dim3((unsigned)(tiles - first < RUN ? tiles - first : RUN)));
     }
 }
-template <int FA, int FB, int TM, int TN, int WM, int WN, int SK, int AHEAD> void tile_launch(ProductArgs p, hipStream_t st) {
+template <int FA, int FB, int TM, int TN, int WM, int WN, int SK> void tile_launch(ProductArgs p, hipStream_t st) {
     in_runs(p, (((long)p.n + TM - 1) / TM) * (((long)p.m + TN - 1) / TN),
-            [&](dim3 grid) { hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK, AHEAD>), grid, dim3(64 * WM * WN), 0, st, p); });
+            [&](dim3 grid) { hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK>), grid, dim3(64 * WM * WN), 0, st, p); });
 }
 // Which kernel: by how many workgroups the sizes make of the chip, measured at d = 2048 unless said otherwise (us, E4M3 x E2M1).
 //  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 408 against
@@ -676,16 +677,16 @@ template <int FA, int FB> int product(bts_context *ctx, ProductArgs p, hipStream
     }
     if constexpr (BIG) {
         if ((t256 + cus - 1) / cus * cus * 4 * 2 <= t128 * 3) {
-            tile_launch<FA, FB, 256, 256, FA == E2M1 ? 2 : 4, FA == E2M1 ? 4 : 2, 1, 1>(p, st);
+            tile_launch<FA, FB, 256, 256, FA == E2M1 ? 2 : 4, FA == E2M1 ? 4 : 2, 1>(p, st);
             BTS_LAUNCH_CHECK();
             return BTS_OK;
         }
     }
-    if (p.n <= 32) tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
-    else if (p.m <= 32) tile_launch<FA, FB, 64, 16, 4, 1, 2, 2>(p, st);
-    else if (t128 >= 2 * cus) tile_launch<FA, FB, 128, 128, 2, 2, SK, 2>(p, st);
-    else if (tiles(64, 64) >= cus) tile_launch<FA, FB, 64, 64, 1, 4, SK, 2>(p, st);
-    else tile_launch<FA, FB, 16, 64, 1, 4, 2, 2>(p, st);
+    if (p.n <= 32) tile_launch<FA, FB, 16, 64, 1, 4, 2>(p, st);
+    else if (p.m <= 32) tile_launch<FA, FB, 64, 16, 4, 1, 2>(p, st);
+    else if (t128 >= 2 * cus) tile_launch<FA, FB, 128, 128, 2, 2, SK>(p, st);
+    else if (tiles(64, 64) >= cus) tile_launch<FA, FB, 64, 64, 1, 4, SK>(p, st);
+    else tile_launch<FA, FB, 16, 64, 1, 4, 2>(p, st);
     BTS_LAUNCH_CHECK();
     return BTS_OK;
 }
