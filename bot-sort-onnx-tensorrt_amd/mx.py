@@ -225,7 +225,8 @@ def mx_quantize(x, fmt: str = "e2m1", out: MxRows = None) -> MxRows:
     lib, ctx, stream = _call(x.device)
     pc, ps = rows._pointers()
     _lib.check(lib.bts_mx_quantize(ctx, p, dt, ld, n, d, f, pc, ps, stream))
-    _written(out)
+    if out is not None:
+        _written(out)
     return rows
 
 
@@ -249,7 +250,9 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
     h = sum_out
     if h is None and (residual is not None or py == px):            # (y in the place of x: h is x as it was)
         h = torch.empty((n, d), dtype=x.dtype, device=x.device)
-    ps, lds = _rows2d(h, "sum_out", x) if h is not None else (None, 0)
+        ps, lds = h.data_ptr(), d
+    else:
+        ps, lds = _rows2d(h, "sum_out", x) if h is not None else (None, 0)
     if fmt is None and out is not None:
         raise _lib.BtsError("out: rows to fill need their fmt")
     f = 0 if fmt is None else _format_code(fmt)
@@ -273,19 +276,21 @@ def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = Fals
     if a.d != b.d or b.device != device:
         raise _lib.BtsError("mx_product: rows of one width on one device expected, got %r and %r" % (a, b))
     n, m = a._n, b._n
-    given = out
-    if out is None:
+    made = out is None
+    if made:
         if dtype is None:
             dtype = torch.float32 if a.fmt == b.fmt == "e2m1" else torch.bfloat16
         code = _dtype_code(dtype)
         out = torch.empty((n, m), dtype=dtype, device=device)
+        po, ld = out.data_ptr(), m
     else:
         code = _dtype_code(_tensor(out, "out").dtype)
         if tuple(out.shape) != (n, m) or out.device != device or dtype not in (None, out.dtype):
             raise _lib.BtsError("out: [%d, %d] on %s%s expected" % (n, m, device, "" if dtype is None else " of %s" % dtype))
-    po, ld = _rows2d(out, "out")
+        po, ld = _rows2d(out, "out")
     lib, ctx, stream = _call(device)
     (ac, as_), (bc, bs) = a._pointers(), b._pointers()
     _lib.check(lib.bts_mx_product(ctx, ac, as_, a._code, n, bc, bs, b._code, m, a.d, float(alpha), 1 if floor_zero else 0, po, code, ld, stream))
-    _written(given)
+    if not made:
+        _written(out)
     return out
