@@ -14,7 +14,7 @@ typedef float v4f __attribute__((ext_vector_type(4)));
 
 // ---- quantisation and back: one thread per 8 elements, four lanes per block, 16 lanes per 128 padded elements ------------------
 // Groups of 16 lanes walk the 128-element pieces of all rows (their number fits 32 bits: the host's check).  Memory bounds both ways:
-// 65536 x 2048 bfloat16 to E2M1, 340 MB, in 77 us (4.4 TB/s), back in 60 us (5.6 TB/s).
+// 65536 x 2048 bfloat16 to E2M1, 340 MB, in 77 us (4.4 TB/s), back in 59 us (5.7 TB/s, the codes still in the last-level cache).
 template <class T, int FMT>
 __global__ __launch_bounds__(256) void k_mx_quantize(const T *__restrict__ x, long ldx, uint32_t pieces, uint32_t row_pieces, int d,
                                                      uint8_t *__restrict__ codes, uint8_t *__restrict__ scales) {
@@ -127,7 +127,7 @@ template <class T, bool WHOLE> __device__ __forceinline__ void norm_emit(const N
 
 // TPR threads per row, CH pieces of 8 elements a thread: the row stays in registers between the sum and the output, so x and residual
 // are read once.  CH = 0: rows beyond 8192 elements, in two passes; the second reads the stored sum, or x and residual again.
-// One pass over memory bounds it: 32768 x 4096 bfloat16 with residual and weight, 0.94 GB in 177 us (5.3 TB/s).
+// One pass over memory bounds it: 32768 x 4096 bfloat16 with residual and weight, 0.94 GB in 164 us (5.7 TB/s; 178 between decodings).
 template <class T, int TPR, int CH, bool WHOLE>
 __global__ __launch_bounds__(256) void k_rms_norm(NormArgs<T> a) {
     __shared__ double part[4];
@@ -257,8 +257,8 @@ template <class T> __device__ __forceinline__ void epilogue4(const ProductArgs &
 }
 
 // A workgroup of 4 wavefronts computes one 16 x 16 tile straight from memory; each wavefront takes a quarter of the row, and the parts are
-// added through LDS in a fixed order.  For few tiles, where the length of a row is what takes time (1 x 2000 x 2048: 3.5 us against 5.2
-// with LDS tiles; 1 x 300 x 8192: 6.7 against 12.2), and for sizes beyond the tiles' 32-bit offsets.
+// added through LDS in a fixed order.  For few tiles, where the length of a row is what takes time (1 x 2000 x 2048: 3.4 us against 5.1
+// with LDS tiles; 1 x 300 x 8192: 6.6 against 12.2), and for sizes beyond the tiles' 32-bit offsets.
 template <int FA, int FB>
 __global__ __launch_bounds__(256) void k_mx_direct(ProductArgs p) {
     __shared__ v4f part[3][64];
@@ -303,7 +303,7 @@ struct TileRows {
 
 // Lane l has the four scale bytes of row l; after this it has byte l >> 4 of the rows l & 15, that + 16, + 32 and + 48: those of its elements
 // in four fragments.  (A 4 x 4 transposition of bytes over lanes 16 apart, so that they go to LDS a word at a time instead of four bytes:
-// 10000 x 2000 x 8192 took 132 us instead of 138.)
+// 4 % of the time of 10000 x 2000 x 8192.)
 __device__ __forceinline__ uint32_t transpose_bytes(uint32_t w, int lane) {
     const auto far = __builtin_amdgcn_permlane32_swap(w, w, false, false);        // [0]: the word of the lane's pair with bit 5 clear, [1]: set
     w = __builtin_amdgcn_perm(far[1], far[0], lane & 32 ? 0x07060302u : 0x05040100u);
@@ -414,12 +414,14 @@ __device__ __forceinline__ void write_tile(const ProductArgs &p, const v4f (&acc
 // (Fragments straight from memory would be 16 rows x 64 bytes a load with the lanes of a row 16 apart: a quarter of the load path's rate.)
 // With 8 wavefronts (two a SIMD) the second four run one phase behind the first: while one of a SIMD's two wavefronts multiplies, the
 // other fetches its fragments, stores the next stage and issues the loads of the one after; barriers keep the two in step.  With 4
-// wavefronts a stage has one barrier, a depth's fragments are read while the one before it is multiplied (1000 x 1000 x 1000: 5.2 us
-// against 6.6 with both in turn), and the workgroups of a CU overlap.
-// What bounds it (128 x 128, E2M1 x E2M1, 10240 x 2048 x 8192, 130 us): the matrix instructions, the fragment reads and the output take 77,
-// the writes to LDS 25 more, the loads 28; the reads cost nothing beside the instructions.  A round of tiles computes and then stores together, so the output of
-// 10000 x 2000 float32 (17 us) comes on top of the loop (14 us per 1024 elements of depth).  256 x 256 tiles of E4M3 x E2M1, 16384 x 8192 x
-// 4096: 440 us, 2.5 PFLOP/s; the same with zeros in all codes is a quarter faster, that is the card's power limit.
+// wavefronts a stage has one barrier, a depth's fragments are read while the one before it is multiplied (a fifth faster at 1000 x 1000 x
+// 1000 than both in turn: 5.4 us), and the workgroups of a CU overlap.
+// What bounds it: waiting.  128 x 128, E2M1 x E2M1, 10240 x 2048 x 8192, 129 us: the matrix units are busy for 33 % of the cycles, the LDS for
+// 38 %; without the loop's loads it takes 101 us, without its writes to LDS as well 76 (and 82 without the fragment reads as well: the
+// parts overlap and do not add up).  Half of the requests that reach L2 are for scale bytes, a word a row and depth.  With an E4M3 operand
+// (one depth a stage) 41 %; 256 x 256 tiles keep the matrix units busy for 74 to 77 % and take 415 us for E4M3 x E2M1, 16384 x 8192 x 4096
+// (2.6 PFLOP/s; 367 with zeros in all codes, which power does not hold back).  A round of tiles computes and then stores together, so
+// the output of 10000 x 2000 float32 (80 MB) comes on top of the loop.
 template <int FA, int FB, int TM, int TN, int WM, int WN, int SK>
 __global__ __launch_bounds__(64 * WM * WN, 2) void k_mx_tile(ProductArgs p) {
     constexpr int THREADS = 64 * WM * WN, RT = TM / WM / 16, CT = TN / WN / 16;
@@ -653,22 +655,25 @@ template <int FA, int FB, int TM, int TN, int WM, int WN, int SK> void tile_laun
     in_runs(p, (((long)p.n + TM - 1) / TM) * (((long)p.m + TN - 1) / TN),
             [&](dim3 grid) { hipLaunchKernelGGL((k_mx_tile<FA, FB, TM, TN, WM, WN, SK>), grid, dim3(64 * WM * WN), 0, st, p); });
 }
-// Which kernel: by how many workgroups the sizes make of the chip, measured at d = 2048 unless said otherwise (us, E4M3 x E2M1).
-//  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 408 against
-//    613; 6000 x 2000, one round: 28 against 35; 10000 x 2000, 320 tiles in two rounds: 53 against 55, with E2M1 on both sides 55 against
-//    43).  Two E4M3 operands' images of 256 rows do not fit.
-//  - 128 x 128 tiles from two a CU on (2000 x 2000 x 1024, one a CU: 12.2 against 11.7 with 64 x 64 ones).
-//  - 64 x 64 tiles from one a CU on (48 x 65536: 20; 1000 x 1000 x 1000: 5.9), below that 16 x 64 ones (for these two 27 and 6.6; 200 x 2000 x
-//    1024: 4.8 against 5.3), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.7 against 18).
-//  - 16 x 16 tiles with the row split where there are fewer of them than CUs (1 x 2000: 3.5 against 5.2; 16 x 3000 x 512: 2.9 against 3.6;
-//    300 x 300 x 1000, one and a half a CU: 4.6 against 4.1).
+// Which kernel: by how many workgroups the sizes make of the chip, one border for all pairs of formats and all d.  Times in us of the kernel
+// back to back; E4M3 x E2M1 and d = 2048 where nothing else is said.
+//  - 256 x 256 tiles take a CU each, in whole rounds of the CUs, counted at 2/3 of the time per area of 128 x 128 ones (16384 x 8192 x 4096: 415
+//    against 609; 6000 x 2000, one round: 27 against 34).  E2M1 x E2M1 gains less: 350 against 383, and 28 against 27.  10000 x 2000, 320
+//    tiles in two rounds, goes to 128 x 128: 49 against 51, E2M1 x E4M3 49 against 53, E2M1 x E2M1 39 against 53 -- at d = 8192, 195 against
+//    162, 192 against 160 and 125 against 155, so a border that knew the pair and d would give the first two of these to 256 x 256.
+//    Two E4M3 operands: the fragments do not fit the registers (36 spilled): 16384 x 8192 x 4096 1131 against 712 with 128 x 128.
+//  - 128 x 128 tiles from two a CU on (2000 x 2000 x 1024, one a CU: 12.1 against 11.4 with 64 x 64 ones).
+//  - 64 x 64 tiles from one a CU on (48 x 65536: 18; 1000 x 1000 x 1000: 5.8), below that 16 x 64 ones (for these two 23 and 6.5; 200 x 2000 x
+//    1024: 4.7 against 5.2), and these too where one side has up to 32 rows, lying along the other (1 x 65536: 12.4 against 17).
+//  - 16 x 16 tiles with the row split where there are fewer of them than CUs (1 x 2000: 3.4 against 5.1; 16 x 3000 x 512: 2.9 against 3.4;
+//    300 x 300 x 1000, one and a half a CU: 4.5 against 4.1; long rows do not move this border: 64 x 2000 x 8192 19.7 against 12.6).
 template <int FA, int FB> int product(bts_context *ctx, ProductArgs p, hipStream_t st) {
     const auto tiles = [&](long a, long b) { return ((p.n + a - 1) / a) * ((p.m + b - 1) / b); };
     const long cus = ctx->n_cu, t256 = tiles(256, 256), t128 = tiles(128, 128), most = 1L << 31;
     BTS_REQUIRE(tiles(16, 16) < most, "n * m: too many tiles for one launch");
     constexpr int SK = FA == E2M1 && FB == E2M1 ? 2 : 1;      // 128 bytes a row and stage
     constexpr bool BIG = FA == E2M1 || FB == E2M1;
-    // 32-bit offsets inside a tile: 256 rows of codes, 16 rows of the output
+    // 32-bit offsets inside a tile: 256 rows of codes, 16 rows of the output (counted in 4-byte elements whatever the type)
     const bool fits = (long)p.steps * 128 * 256 < most && p.ld * 4 * 16 < most && p.n < most - 256 && p.m < most - 256;
     if (!fits || tiles(16, 16) < cus) {
         in_runs(p, tiles(16, 16), [&](dim3 grid) { hipLaunchKernelGGL((k_mx_direct<FA, FB>), grid, dim3(256), 0, st, p); });
@@ -783,7 +788,7 @@ int bts_mx_product(bts_context *ctx, const uint8_t *a_codes, const uint8_t *a_sc
     BTS_REQUIRE(ctx && n >= 0 && m >= 0 && d > 0 && d <= MOST_WIDE && ld >= m, "ctx, n, m, d (1 .. 2^30), ld < m");
     BTS_REQUIRE(known_format(a_format) && known_format(b_format) && known_dtype(out_dtype), "unknown format / type");
     BTS_REQUIRE(out_dtype != BTS_F32 || (a_format == E2M1 && b_format == E2M1),
-                "a float32 output needs two E2M1 operands (products with an E4M3 operand carry about 16 bits)");
+                "a float32 output needs two E2M1 operands (with an E4M3 operand, products are aligned to the largest with about 13 bits behind it)");
     BTS_REQUIRE(fabs(alpha) <= 3.4028234663852886e38 && ((float)alpha != 0.0f || alpha == 0.0), "alpha must be a float32: finite, and not too small for one");
     BTS_ON_DEVICE(ctx);
     if (n == 0 || m == 0) return BTS_OK;
