@@ -3,6 +3,7 @@ them, and their product -- `cosine_similarity` for galleries that are kept quant
 
 Unlike the NumPy-in / NumPy-out functions of `matching`, everything here takes and returns DEVICE tensors and only enqueues work on
 torch's current stream of their device (like `DeviceTracker.step`): no copies, no synchronisation, safe to capture in a graph.
+Tensors handed in to be filled may not share memory with inputs, except where a call says so; nothing here forms gradients.
 """
 from __future__ import annotations
 
@@ -266,7 +267,7 @@ def rms_norm_mx(x, residual=None, weight=None, eps: float = 1e-6, fmt: str = "e4
 
 
 def mx_product(a: MxRows, b: MxRows, alpha: float = 1.0, floor_zero: bool = False, dtype=None, out=None):
-    """[len(a), len(b)] of alpha * <a_i, b_j>; floor_zero: max(0, .), the similarity of `cosine_similarity` for unit rows.
+    """[len(a), len(b)] of alpha (a float32) * <a_i, b_j>; floor_zero: max(0, .), the similarity of `cosine_similarity` for unit rows.
 
     `dtype`: float32 (the default) where both are e2m1; float16 / bfloat16 for any (the default with an e4m3 operand is bfloat16).
     `out`: a matrix to fill (its type counts; rows may be strided)."""
